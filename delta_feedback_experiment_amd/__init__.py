@@ -11,7 +11,9 @@ RMSNorm with a sigmoid output gate (``fla_ops.py:572-657``), the control
 activations with their packed gradient (:mod:`.controls`; the decay
 expansion runs inside the gate kernel, ``chunk_pkda(..., decay_up=...)``), and
 the slot-pool serving path that connects a cached prefill to the decode step
-(:mod:`.serve`).  Nothing here falls back to the CPU: without a HIP device and
+(:mod:`.serve`).  For the trunk's attention layers a server finds the paged
+key/value cache and the attention over it (:mod:`.paged`), and for its last
+step the sampling of the next token (:mod:`.sample`).  Nothing here falls back to the CPU: without a HIP device and
 the built library every operator raises.
 """
 
@@ -20,8 +22,11 @@ from .controls import pkda_controls
 from .conv import pkda_qkv_conv
 from .norm_gate import pkda_norm_gate
 from .ops import pkda_recurrence
+from .paged import PagedKV, paged_append_, paged_attention
 from .pkda import fused_recurrent_pkda, pkda_decode_step_
+from .sample import sample_tokens
 from .serve import DecodePool, pkda_prefill_, pkda_qkv_conv_cached_
 
-__all__ = ["DecodePool", "chunk_pkda", "fused_recurrent_pkda", "pkda_controls", "pkda_decode_step_",
-           "pkda_norm_gate", "pkda_prefill_", "pkda_qkv_conv", "pkda_qkv_conv_cached_", "pkda_recurrence"]
+__all__ = ["DecodePool", "PagedKV", "chunk_pkda", "fused_recurrent_pkda", "paged_append_", "paged_attention",
+           "pkda_controls", "pkda_decode_step_", "pkda_norm_gate", "pkda_prefill_", "pkda_qkv_conv",
+           "pkda_qkv_conv_cached_", "pkda_recurrence", "sample_tokens"]

@@ -1,8 +1,10 @@
-"""ctypes binding of ``libpkda_gfx950.so`` (the C ABI in ``include/pkda_gfx950.h``).
+"""ctypes binding of ``libpkda_gfx950.so`` (the C ABI in ``include/pkda_gfx950.h``
+and, for the serving operators, ``include/serve/pkda_serve_gfx950.h``).
 
-The structs below mirror the header field for field; ``check_abi`` compares
-their sizes with the library's own ``pkda_args_size`` so a drifted mirror
-fails at load time instead of passing garbage to a kernel.
+The structs below mirror the headers field for field; ``lib`` compares
+their sizes with the library's own ``pkda_args_size`` and
+``pkda_serve_args_size`` so a drifted mirror fails at load time instead of
+passing garbage to a kernel.
 """
 
 from __future__ import annotations
@@ -24,6 +26,7 @@ STAGE_FWD_STATE = 2
 STAGE_BWD_STATE = 1
 STAGE_BWD_CHUNK = 2
 ABI_VERSION = 14
+SERVE_ABI_VERSION = 1
 
 
 class RecurrentArgs(ctypes.Structure):
@@ -137,8 +140,46 @@ class ControlsArgs(ctypes.Structure):
     ]
 
 
+_PAGED_COMMON = [
+    ("num_seqs", c_int32), ("num_tokens", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32),
+    ("head_dim", c_int32), ("page_size", c_int32), ("max_pages", c_int32),
+    ("num_pages", c_int64), ("table_stride", c_int64),
+    ("cu_seqlens", c_void_p), ("seq_lens", c_void_p), ("page_table", c_void_p),
+]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [("struct_size", c_int32), ("dtype", c_int32)] + _PAGED_COMMON + [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+        ("q_stride", c_int64), ("k_stride", c_int64), ("v_stride", c_int64),
+        ("q_out", c_void_p), ("k_pages", c_void_p), ("v_pages", c_void_p),
+        ("k_page_stride", c_int64), ("v_page_stride", c_int64),
+        ("cos", c_void_p), ("sin", c_void_p), ("rotary_dim", c_int32), ("interleaved", c_int32),
+        ("rope_rows", c_int64),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [("struct_size", c_int32), ("dtype", c_int32)] + _PAGED_COMMON + [
+        ("q", c_void_p), ("q_stride", c_int64), ("k_pages", c_void_p), ("v_pages", c_void_p),
+        ("k_page_stride", c_int64), ("v_page_stride", c_int64), ("scale", c_float),
+        ("o", c_void_p), ("lse", c_void_p), ("workspace", c_void_p),
+    ]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_int32), ("dtype", c_int32), ("rows", c_int32), ("vocab", c_int32),
+        ("logits", c_void_p), ("logits_stride", c_int64), ("noise", c_void_p), ("noise_stride", c_int64),
+        ("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p), ("min_p", c_void_p),
+        ("temperature_all", c_float), ("top_k_all", c_int32), ("top_p_all", c_float), ("min_p_all", c_float),
+        ("token", c_void_p), ("logprob", c_void_p),
+    ]
+
+
 _ARG_KINDS = {0: RecurrentArgs, 1: GateArgs, 2: PrecondArgs, 3: ChunkFwdArgs, 4: ChunkBwdArgs, 5: QkvConvArgs,
               6: NormGateArgs, 7: ControlsArgs}
+_SERVE_ARG_KINDS = {0: PagedAppendArgs, 1: PagedAttentionArgs, 2: SampleArgs}
 _LIB: ctypes.CDLL | None = None
 
 
@@ -191,6 +232,8 @@ def lib() -> ctypes.CDLL:
         ("pkda_qkv_conv_fwd", QkvConvArgs), ("pkda_qkv_conv_bwd", QkvConvArgs),
         ("pkda_norm_gate_fwd", NormGateArgs), ("pkda_norm_gate_bwd", NormGateArgs),
         ("pkda_controls_fwd", ControlsArgs), ("pkda_controls_bwd", ControlsArgs),
+        ("pkda_paged_append", PagedAppendArgs), ("pkda_paged_attention", PagedAttentionArgs),
+        ("pkda_sample", SampleArgs),
     ):
         fn = getattr(handle, name, None)
         if fn is not None:
@@ -204,10 +247,19 @@ def lib() -> ctypes.CDLL:
     handle.pkda_controls_workspace.argtypes = [c_int64, c_int32]
     handle.pkda_chunk_table.restype = c_int32
     handle.pkda_chunk_table.argtypes = [c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]
+    handle.pkda_serve_abi_version.restype = c_int32
+    handle.pkda_serve_args_size.restype = c_int64
+    handle.pkda_serve_args_size.argtypes = [c_int32]
+    handle.pkda_paged_attention_workspace.restype = c_int64
+    handle.pkda_paged_attention_workspace.argtypes = [POINTER(PagedAttentionArgs)]
     if handle.pkda_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libpkda ABI {handle.pkda_abi_version()} != binding ABI {ABI_VERSION}")
-    for kind, struct in _ARG_KINDS.items():
-        size = handle.pkda_args_size(kind)
+    if handle.pkda_serve_abi_version() != SERVE_ABI_VERSION:
+        raise RuntimeError(f"libpkda serving ABI {handle.pkda_serve_abi_version()} != binding {SERVE_ABI_VERSION}")
+    kinds = [(handle.pkda_args_size, k, s) for k, s in _ARG_KINDS.items()]
+    kinds += [(handle.pkda_serve_args_size, k, s) for k, s in _SERVE_ARG_KINDS.items()]
+    for size_of, kind, struct in kinds:
+        size = size_of(kind)
         if size >= 0 and size != ctypes.sizeof(struct):
             raise RuntimeError(f"{struct.__name__}: binding size {ctypes.sizeof(struct)} != library {size}")
     runtimes = _hip_runtimes_loaded()

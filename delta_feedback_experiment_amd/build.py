@@ -1,4 +1,4 @@
-"""Build ``libpkda_gfx950.so`` from ``csrc/*.hip`` for gfx950, in-tree.
+"""Build ``libpkda_gfx950.so`` from ``csrc/*.hip`` and ``csrc/serve/*.hip`` for gfx950, in-tree.
 
     python -m delta_feedback_experiment_amd.build
 
@@ -66,14 +66,14 @@ def library_path() -> Path:
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile every ``csrc/*.hip`` and link the shared library; return its path."""
-    sources = sorted(CSRC.glob("*.hip"))
+    """Compile every ``csrc/**/*.hip`` and link the shared library; return its path."""
+    sources = sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("serve/*.hip"))
     if not sources:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     BUILD.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
     hipcc = _hipcc()
-    headers = sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
+    headers = sorted(CSRC.glob("**/*.h")) + sorted(INCLUDE.glob("*.h"))
 
     def compile_one(src: Path) -> Path:
         obj = BUILD / (src.stem + ".o")
