@@ -1,10 +1,46 @@
 // Attention of new tokens over a paged key/value cache (gfx950).
+//
+// Rows.  The group = q_heads / kv_heads query heads of one key/value head share
+// its keys, so a workgroup's tile is rows of (token, query head of the group)
+// of one sequence, tokens slowest: a single token fills group rows, a chunk
+// any number.  Scores, softmax and output run in one pass over the keys with
+// the row's running maximum m and sum l (base 2, FP32):
+//   m' = max(m, max_s S),  p = 2^(S - m'),  l = l 2^(m - m') + sum_s p,
+//   O = O 2^(m - m') + p V,   o = O / l,  lse = (m + log2 l) ln 2.
+//
+// Products.  Both are taken transposed, S^T = K Q^T and O^T = V^T P^T, as
+// 32x32 MFMA tiles.  A lane then holds one query row (its column) and 16 of a
+// tile's 32 keys, so a row's maximum and sum are a lane's own and one exchange
+// between the wave's halves, the rescaling of O is a multiply by the lane's own
+// factor, and P^T is already the second product's operand: the accumulator's
+// key order, 8 (r / 4) + 4 half + r % 4 for register r, is the order in which
+// the product reads V's rows.  K, Q and V keep their 16-byte chunks: chunk 2 i +
+// half of a row is operand i of the lane's half (BF16: one 32x32x16 step; FP32:
+// four 32x32x2 steps).
+//
+// Two kernels.  Up to 32 rows of a tile (decode): four waves take 32 keys each
+// in turn, each with its own m, l and O, and join at the end; keys go straight
+// from memory to operand registers, values through a wave's own piece of LDS
+// (the transposing reads), the next tile's loads in flight during a tile's
+// arithmetic.  More rows (a chunk): four waves of 32 rows share tiles of 64 keys
+// staged in LDS, double-buffered.  Where rows are few, a sequence's keys are
+// split over workgroups and a third kernel joins the parts.
+#include <math.h>
+
 #include "paged_common.h"
 
 namespace pkda {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMinChunk = 128;  // keys of a split, at least
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 struct AttnParams {
   PagedSeqs s;
@@ -12,83 +48,694 @@ struct AttnParams {
   int64_t q_stride;
   const void *k_pages, *v_pages;
   int64_t k_page_stride, v_page_stride;
-  int q_heads, kv_heads, group;
-  float scale2;  // scale log2 e: the softmax is taken in base 2
+  int q_heads, kv_heads;
+  FastDiv group;
+  float scale2;  // |scale| log2 e: the softmax is taken in base 2
+  bool negate;   // scale < 0: queries are negated
+  int splits;
   void* o;
   float* lse;
+  float* part_o;   // [splits][num_tokens * q_heads][head_dim]
+  float* part_ml;  // [splits][num_tokens * q_heads][2]
 };
 
-// One wave a (token, query head): a lane scores one of 64 positions, then owns
-// D / 64 (at D = 32: one of 32) channels of the output.
+template <typename T, int D> struct Geo {
+  static constexpr int RB = D * (int)sizeof(T);  // bytes of a row
+  static constexpr int NC = RB / 16;             // its chunks
+  static constexpr int EC = 16 / (int)sizeof(T);
+  static constexpr int NP = NC / 2;              // operands of a lane: every other chunk
+  static constexpr int DT = D / 32;              // 32-channel tiles of the output
+};
+
+// Rows lie in LDS with chunk c at place c ^ swizzle(row): the 8 or 16 rows that
+// one phase of an operand read touches, and the four rows of a transposing
+// read, then lie in different banks (rows are 64, 128, 256 or 512 bytes).
+template <int RB>
+__device__ __forceinline__ int swizzle(int r) {
+  if constexpr (RB >= 256) return ((r & 3) << 1) | ((r >> 2) & 1) | (((r ^ (r >> 3)) & 1) << 3);
+  else if constexpr (RB == 128) return ((r & 2) << 1) | (((r ^ (r >> 3)) & 1) << 1) | ((r >> 2) & 1);
+  else return ((r ^ (r >> 2)) & 2) | ((r >> 2) & 1);
+}
+template <int RB>
+__device__ __forceinline__ int lds_chunk(int row, int chunk) {  // byte offset
+  return row * RB + ((chunk ^ swizzle<RB>(row)) << 4);
+}
+
+// acc += A B over one chunk pair; lane: row / column lane & 31, the half's chunk.
+template <typename T>
+__device__ __forceinline__ void mma_chunk(f32x16& acc, const uint4& a, const uint4& b) {
+  if constexpr (sizeof(T) == 2) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  } else {
+    const f32x4_t x = __builtin_bit_cast(f32x4_t, a), y = __builtin_bit_cast(f32x4_t, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], acc, 0, 0, 0);
+  }
+}
+
+// o[dt] += V^T P^T over the 32 keys of the rows at v (LDS, swizzled), P^T in
+// the scores' registers.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void paged_attention_rows_kernel(AttnParams p) {
-  __shared__ float s_q[kThreads / 64][D];
-  __shared__ float s_p[kThreads / 64][64];
-  __shared__ int64_t s_row[kThreads / 64][64];
+__device__ __forceinline__ void mma_values(f32x16 (&o)[D / 32], const char* v, int row0, const f32x16& s, int lane) {
+  using G = Geo<T, D>;
+  if constexpr (sizeof(T) == 2) {
+    const int g = lane >> 4, i = lane & 15;
+    const int key0 = row0 + 4 * (g >> 1) + (i >> 2);
+    const int chunk = 2 * (g & 1) + ((i & 3) >> 1), within = 8 * (i & 1);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      bf16x8 p;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = static_cast<__bf16>(s[8 * j + e]);
+      const int ra = key0 + 16 * j, rb = ra + 8;
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt) {
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(v + lds_chunk<G::RB>(ra, 4 * dt + chunk) + within));
+        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(v + lds_chunk<G::RB>(rb, 4 * dt + chunk) + within));
+        const bf16x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p, o[dt], 0, 0, 0);
+      }
+    }
+  } else {
+    const int half = lane >> 5, c = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int key = row0 + 8 * (r >> 2) + 4 * half + (r & 3);
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt) {
+        const float a = *reinterpret_cast<const float*>(v + lds_chunk<G::RB>(key, 8 * dt + (c >> 2)) + 4 * (c & 3));
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[r], o[dt], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// The wave's other half's value at the same column, joined by f.
+template <typename F>
+__device__ __forceinline__ float join_halves(float x, F f) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The numbers of a chunk that are not finite become zero; whether there were any.
+template <typename T>
+__device__ __forceinline__ bool clear_nonfinite(uint4& x) {
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      if ((w[i] & 0x7f80u) == 0x7f80u) { any = true; w[i] &= 0xffff0000u; }
+      if ((w[i] & 0x7f800000u) == 0x7f800000u) { any = true; w[i] &= 0xffffu; }
+    } else {
+      if ((w[i] & 0x7f800000u) == 0x7f800000u) { any = true; w[i] = 0; }
+    }
+  }
+  x = make_uint4(w[0], w[1], w[2], w[3]);
+  return any;
+}
+
+// A tile of M rows of one sequence.
+struct Tile {
+  SeqSpan span;
+  int n, row0, rows;  // rows: of the sequence, from its first new token
+  int first, last;    // positions of the tile's first and last row (negative: none)
+  int keys;           // what the tile sees: last + 1, or 0
+  int chunk;          // keys of a split
+  bool direct;        // the sequence is not split: this workgroup has the whole softmax
+};
+
+__device__ __forceinline__ int split_chunk(int len, int splits) {
+  const int c = (len + splits - 1) / splits;
+  return max(kMinChunk, (c + kMinChunk - 1) / kMinChunk * kMinChunk);
+}
+
+// Tiles are numbered through the sequences with room for one that is not full
+// each: sequence n's begin at floor(first row / M) + n, which holds ceil(rows /
+// M) of them and needs no sum over the sequences before.
+__host__ __device__ inline int64_t tile_bound(int64_t tokens, int64_t seqs, int64_t group, int M, bool packed) {
+  return packed ? tokens * group / M + seqs + 1 : seqs * ((group + M - 1) / M);
+}
+template <int M>
+__device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& tile) {
+  const int group = (int)p.group.d;
+  int local;
+  if (p.s.cu) {
+    const auto begin = [&](int n) -> int64_t {
+      return (n == 0 ? 0 : (int64_t)clamp_int(p.s.cu[n], 0, p.s.num_tokens) * group / M) + n;
+    };
+    tile.n = wave_upper(p.s.num_seqs, t, begin);
+    local = (int)(t - begin(tile.n));
+  } else {
+    const int per = (group + M - 1) / M;
+    tile.n = (int)(t / per);
+    local = (int)(t - (int64_t)tile.n * per);
+  }
+  tile.span = seq_span(p.s, tile.n);
+  const int64_t rows = (int64_t)tile.span.count * group, row0 = (int64_t)local * M;
+  if (row0 >= rows) return false;
+  tile.rows = (int)rows;
+  tile.row0 = (int)row0;
+  const int base = tile.span.len - tile.span.count;
+  tile.first = base + (int)p.group.div((uint32_t)row0);
+  tile.last = base + (int)p.group.div((uint32_t)min(rows - 1, row0 + M - 1));
+  tile.keys = p.s.num_pages == 0 ? 0 : max(0, tile.last + 1);
+  tile.chunk = split_chunk(tile.span.len, p.splits);
+  tile.direct = tile.span.len <= tile.chunk;
+  return true;
+}
+
+// One query row of a lane.
+struct Row {
+  int64_t index;  // token * q_heads + head
+  int pos;        // its position; -1: sees nothing
+  bool live;
+};
+template <typename T, int D>
+__device__ __forceinline__ Row load_row(const AttnParams& p, const Tile& tile, int kvh, int r, int half,
+                                        uint4 (&q)[Geo<T, D>::NP]) {
+  using G = Geo<T, D>;
+  Row row;
+  row.live = r < tile.rows;
+  row.pos = -1;
+  row.index = 0;
+#pragma unroll
+  for (int i = 0; i < G::NP; ++i) q[i] = make_uint4(0, 0, 0, 0);
+  if (row.live) {
+    const int j = (int)p.group.div((uint32_t)r), g = r - j * (int)p.group.d;
+    const int h = kvh * (int)p.group.d + g, t = tile.span.first + j;
+    row.index = (int64_t)t * p.q_heads + h;
+    row.pos = max(-1, tile.span.len - tile.span.count + j);
+    const T* src = static_cast<const T*>(p.q) + t * p.q_stride + (int64_t)h * D + half * G::EC;
+#pragma unroll
+    for (int i = 0; i < G::NP; ++i) q[i] = *reinterpret_cast<const uint4*>(src + 2 * i * G::EC);
+    if (p.negate) {
+      const uint32_t sign = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+#pragma unroll
+      for (int i = 0; i < G::NP; ++i) { q[i].x ^= sign; q[i].y ^= sign; q[i].z ^= sign; q[i].w ^= sign; }
+    }
+  }
+  return row;
+}
+
+// A row's softmax while its keys pass.
+template <int DT> struct Running {
+  float m, l;  // maximum (base 2), and the sum over this half's keys
+  f32x16 o[DT];
+  __device__ __forceinline__ void init() {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  }
+  // scores of N tiles of keys -> their probabilities
+  template <int N>
+  __device__ __forceinline__ void step(f32x16 (&s)[N], float scale2) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+    mx = join_halves(mx, [](float a, float b) { return fmaxf(a, b); }) * scale2;
+    if (__any(mx > m)) {
+      const float mn = fmaxf(m, mx);
+      const float a = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= a;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[n][r] = exp2_fast(__builtin_fmaf(s[n][r], scale2, -base));
+        sum += s[n][r];
+      }
+    l += sum;
+  }
+};
+
+__device__ __forceinline__ int key_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+// What values that are not finite add to the rows that see them (the products
+// ran with zeros there, so that a row that does not see them stays what it is):
+// key by key, a product of those values alone, which only lanes whose row sees
+// the key take.  bad: the tile's keys with such values.
+template <typename T, int D, int N>
+__device__ __forceinline__ void add_nonfinite(f32x16 (&o)[D / 32], const f32x16 (&s)[N], uint64_t bad, const AttnParams& p,
+                                              int n, int kvh, int key0, int pos, int lane) {
+  const int half = lane >> 5;
+  while (bad) {
+    const int i = __builtin_ctzll(bad);
+    bad &= bad - 1;
+    int row;
+    const int page = page_of(p.s, n, key0 + i, &row);
+    if (page < 0) continue;
+    const T* v = static_cast<const T*>(p.v_pages) + page * p.v_page_stride + ((int64_t)row * p.kv_heads + kvh) * D;
+    const int key_half = (i >> 2) & 1, key_r = 4 * ((i & 31) >> 3) + (i & 3);
+    float pr = 0.f;  // the key's probability, in the lanes of its half
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (t == i >> 5 && r == key_r) pr = s[t][r];
+    const bool sees = key0 + i <= pos;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      float x = io<T>::load(v + 32 * dt + (lane & 31));
+      if (half != key_half || fabsf(x) < INFINITY) x = 0.f;
+      f32x16 add;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) add[r] = 0.f;
+      if constexpr (sizeof(T) == 2) {
+        const __bf16 z = static_cast<__bf16>(0.f);
+        add = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf16x8{static_cast<__bf16>(x), z, z, z, z, z, z, z},
+                                                      bf16x8{static_cast<__bf16>(pr), z, z, z, z, z, z, z}, add, 0, 0, 0);
+      } else {
+        add = __builtin_amdgcn_mfma_f32_32x32x2f32(x, pr, add, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] += sees ? add[r] : 0.f;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 32 rows a tile: the keys over the waves.
+// ---------------------------------------------------------------------------
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) void paged_attention_keys_kernel(AttnParams p) {
+  using G = Geo<T, D>;
+  constexpr int OS = D + 4;  // floats between the rows of a wave's output in LDS
+  constexpr int kStage = kWaves * 32 * G::RB, kJoin = kWaves * 32 * OS * 4;
+  __shared__ __align__(16) char s_buf[kStage > kJoin ? kStage : kJoin];
+  __shared__ float s_m[kWaves][32], s_l[kWaves][32];
+
+  const int kvh = blockIdx.x % p.kv_heads;
+  const int rest = blockIdx.x / p.kv_heads;
+  const int split = rest % p.splits;
+  Tile tile;
+  if (!find_tile<32>(p, rest / p.splits, tile)) return;
+  if (p.s.cu && (int64_t)tile.rows > 32) return;  // the other kernel's
+  const int k0 = split * tile.chunk, k1 = min(k0 + tile.chunk, tile.keys);
+  if (split > 0 && (k0 >= tile.keys || tile.direct)) return;
+
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + w;
-  const bool live = row < (int64_t)p.s.num_tokens * p.q_heads;
-  const int t = live ? (int)(row / p.q_heads) : 0, h = live ? (int)(row - (int64_t)t * p.q_heads) : 0;
-  if (!live) return;
-  const int kvh = h / p.group;
+  const int col = lane & 31, half = lane >> 5;
+  uint4 q[G::NP];
+  const Row row = load_row<T, D>(p, tile, kvh, tile.row0 + col, half, q);
+  Running<G::DT> run;
+  run.init();
+
+  char* sv = s_buf + w * 32 * G::RB;
+  const int tiles = k1 > k0 ? (k1 - k0 + 31) / 32 : 0;
+  const T* kb = static_cast<const T*>(p.k_pages) + (int64_t)kvh * D + half * G::EC;
+  const T* vb = static_cast<const T*>(p.v_pages) + (int64_t)kvh * D + half * G::EC;
+  const int row_stride = p.kv_heads * D;
+
+  // page and row of this lane's key of tile t
+  const auto look = [&](int t, int& r) -> int {
+    const int key = k0 + 32 * t + col;
+    const int page = page_of(p.s, tile.n, min(key, k1 - 1), &r);
+    return key < k1 ? page : -1;
+  };
+  uint4 k[G::NP], v[G::NP];
+  const auto load = [&](int page, int r) {
+    const int64_t at = page < 0 ? 0 : page, off = page < 0 ? 0 : (int64_t)r * row_stride;
+    const T* ks = kb + at * p.k_page_stride + off;
+    const T* vs = vb + at * p.v_page_stride + off;
+#pragma unroll
+    for (int i = 0; i < G::NP; ++i) k[i] = *reinterpret_cast<const uint4*>(ks + 2 * i * G::EC);
+#pragma unroll
+    for (int i = 0; i < G::NP; ++i) v[i] = *reinterpret_cast<const uint4*>(vs + 2 * i * G::EC);
+  };
+
+  int page = -1, page1 = -1, r0 = 0, r1 = 0;
+  if (w < tiles) {
+    page = look(w, r0);
+    if (w + kWaves < tiles) page1 = look(w + kWaves, r1);
+    load(page, r0);
+  }
+  for (int t = w; t < tiles; t += kWaves) {
+    const int key0 = k0 + 32 * t;
+    const uint32_t there = (uint32_t)__ballot(page >= 0);
+    f32x16 s[1];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < G::NP; ++i) mma_chunk<T>(s[0], k[i], q[i]);
+    // values to LDS: rows that are not there as zeros, and in a tile that some
+    // row sees only part of, whatever is not finite
+    const bool partial = key0 + 31 > tile.first;
+    uint32_t bad = 0;
+    if (there != 0xffffffffu) {
+      if (page < 0)
+#pragma unroll
+        for (int i = 0; i < G::NP; ++i) v[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (partial && tile.first != tile.last) {
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < G::NP; ++i) any |= clear_nonfinite<T>(v[i]);
+      const uint64_t b = __ballot(any);
+      bad = (uint32_t)b | (uint32_t)(b >> 32);
+    }
+#pragma unroll
+    for (int i = 0; i < G::NP; ++i) *reinterpret_cast<uint4*>(sv + lds_chunk<G::RB>(col, 2 * i + half)) = v[i];
+    page = page1;
+    if (t + kWaves < tiles) {
+      load(page1, r1);
+      if (t + 2 * kWaves < tiles) page1 = look(t + 2 * kWaves, r1);
+    }
+    if (partial || there != 0xffffffffu) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = key_of(r, half);
+        if (key0 + i > row.pos || !((there >> i) & 1)) s[0][r] = -INFINITY;
+      }
+    }
+    run.step(s, p.scale2);
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    mma_values<T, D>(run.o, sv, 0, s[0], lane);
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    if (bad) add_nonfinite<T, D, 1>(run.o, s, bad, p, tile.n, kvh, key0, row.pos, lane);
+  }
+
+  // the waves' parts: a common maximum, then a sum over the waves in order
+  const float l = join_halves(run.l, [](float a, float b) { return a + b; });
+  if (half == 0) {
+    s_m[w][col] = run.m;
+    s_l[w][col] = l;
+  }
+  __syncthreads();
+  const int live = min(32, tile.rows - tile.row0);
+  {
+    float m = s_m[0][col];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, s_m[i][col]);
+    const float a = exp2_fast(run.m - (m == -INFINITY ? 0.f : m));
+    if (col < live) {
+      float* so = reinterpret_cast<float*>(s_buf) + (w * 32 + col) * OS;
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+          *reinterpret_cast<float4*>(so + 32 * dt + key_of(r, half)) =
+              make_float4(run.o[dt][r] * a, run.o[dt][r + 1] * a, run.o[dt][r + 2] * a, run.o[dt][r + 3] * a);
+    }
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < live * (D / 4); x += kThreads) {
+    const int i = x / (D / 4), c = 4 * (x % (D / 4));
+    float m = s_m[0][i];
+#pragma unroll
+    for (int j = 1; j < kWaves; ++j) m = fmaxf(m, s_m[j][i]);
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < kWaves; ++j) {
+      sum += s_l[j][i] * exp2_fast(s_m[j][i] - (m == -INFINITY ? 0.f : m));
+      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(s_buf) + (j * 32 + i) * OS + c);
+      acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
+    }
+    const int r = tile.row0 + i, j = (int)p.group.div((uint32_t)r);
+    const int64_t out = (int64_t)(tile.span.first + j) * p.q_heads + kvh * (int)p.group.d + (r - j * (int)p.group.d);
+    if (tile.direct) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      store4(static_cast<T*>(p.o) + out * D + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+      if (c == 0) p.lse[out] = (m + __log2f(sum)) * 0.693147180559945309f;
+    } else {
+      const int64_t part = (int64_t)split * p.s.num_tokens * p.q_heads + out;
+      *reinterpret_cast<float4*>(p.part_o + part * D + c) = acc;
+      if (c == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, sum);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// More rows a sequence: 128 rows a tile over the waves, keys staged for all.
+// ---------------------------------------------------------------------------
+constexpr int kRowTile = 32 * kWaves;
+constexpr int kKeyTile = 64;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) void paged_attention_rows_kernel(AttnParams p) {
+  using G = Geo<T, D>;
+  constexpr int NI = kKeyTile * G::NC / kThreads;  // chunks of K (and of V) a thread stages
+  constexpr int RI = kThreads / G::NC;             // rows a pass of the workgroup covers
+  constexpr int kTileBytes = kKeyTile * G::RB;
+  __shared__ __align__(16) char s_kv[4 * kTileBytes];  // two stages of K, V
+  __shared__ uint32_t s_bad[3][2];    // tile t % 3: its keys with values that are not finite
+  __shared__ uint32_t s_there[3][2];  // and those that have a page
+
+  const int kvh = blockIdx.x % p.kv_heads;
+  const int rest = blockIdx.x / p.kv_heads;
+  const int split = rest % p.splits;
+  const int64_t bound = tile_bound(p.s.num_tokens, p.s.num_seqs, p.group.d, kRowTile, true);
+  Tile tile;
+  if (!find_tile<kRowTile>(p, bound - 1 - rest / p.splits, tile)) return;  // the longest first
+  if ((int64_t)tile.rows <= 32) return;                                    // the other kernel's
+  const int k0 = split * tile.chunk, k1 = min(k0 + tile.chunk, tile.keys);
+  if (split > 0 && (k0 >= tile.keys || tile.direct)) return;
+
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int col = lane & 31, half = lane >> 5;
+  uint4 q[G::NP];
+  const int wrow0 = tile.row0 + 32 * w;
+  const Row row = load_row<T, D>(p, tile, kvh, wrow0 + col, half, q);
+  // positions of the wave's first and last live row
+  const int base = tile.span.len - tile.span.count;
+  const bool wlive = wrow0 < tile.rows;
+  const int wfirst = wlive ? base + (int)p.group.div((uint32_t)wrow0) : -1;
+  const int wlast = wlive ? base + (int)p.group.div((uint32_t)min(tile.rows - 1, wrow0 + 31)) : -1;
+  Running<G::DT> run;
+  run.init();
+
+  const int tiles = k1 > k0 ? (k1 - k0 + kKeyTile - 1) / kKeyTile : 0;
+  const int srow = tid / G::NC, schunk = tid % G::NC;
+  const T* kb = static_cast<const T*>(p.k_pages) + (int64_t)kvh * D + schunk * G::EC;
+  const T* vb = static_cast<const T*>(p.v_pages) + (int64_t)kvh * D + schunk * G::EC;
+  const int row_stride = p.kv_heads * D;
+
+  int page[NI], prow[NI];
+  const auto look = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int key = k0 + kKeyTile * t + RI * i + srow;
+      const int at = page_of(p.s, tile.n, min(key, k1 - 1), &prow[i]);
+      page[i] = key < k1 ? at : -1;
+    }
+  };
+  uint4 k[NI], v[NI];
+  uint32_t held;  // this thread's staged rows that are there, one bit each
+  const auto load = [&]() {
+    held = 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int64_t at = page[i] < 0 ? 0 : page[i], off = page[i] < 0 ? 0 : (int64_t)prow[i] * row_stride;
+      held |= (page[i] < 0 ? 0u : 1u) << i;
+      k[i] = *reinterpret_cast<const uint4*>(kb + at * p.k_page_stride + off);
+      v[i] = *reinterpret_cast<const uint4*>(vb + at * p.v_page_stride + off);
+    }
+  };
+  const auto stage = [&](int t, int slot) {
+    char* sk = s_kv + (t & 1) * 2 * kTileBytes;
+    const bool check = k0 + kKeyTile * t + kKeyTile - 1 > tile.first;
+    uint32_t bad = 0;
+    if (held != (1u << NI) - 1u) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        if (!((held >> i) & 1)) v[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (check) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) bad |= (clear_nonfinite<T>(v[i]) ? 1u : 0u) << i;
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = RI * i + srow, at = lds_chunk<G::RB>(r, schunk);
+      *reinterpret_cast<uint4*>(sk + at) = k[i];
+      *reinterpret_cast<uint4*>(sk + kTileBytes + at) = v[i];
+      if ((bad >> i) & 1) atomicOr(&s_bad[slot][r >> 5], 1u << (r & 31));
+      if (!((held >> i) & 1) && schunk == 0) atomicAnd(&s_there[slot][r >> 5], ~(1u << (r & 31)));
+    }
+  };
+  if (tid < 6) {
+    s_bad[tid >> 1][tid & 1] = 0;
+    s_there[tid >> 1][tid & 1] = 0xffffffffu;
+  }
+  __syncthreads();
+  if (tiles > 0) {
+    look(0);
+    load();
+    if (tiles > 1) look(1);
+    stage(0, 0);
+  }
+  __syncthreads();
+  int slot = 0;
+  for (int t = 0; t < tiles; ++t) {
+    const int key0 = k0 + kKeyTile * t, next = slot == 2 ? 0 : slot + 1, free = next == 2 ? 0 : next + 1;
+    if (tid < 2) {  // tile t + 2's, read last before the barrier that ended tile t - 1
+      s_bad[free][tid] = 0;
+      s_there[free][tid] = 0xffffffffu;
+    }
+    if (t + 1 < tiles) {
+      load();
+      if (t + 2 < tiles) look(t + 2);
+    }
+    const char* sk = s_kv + (t & 1) * 2 * kTileBytes;
+    const uint64_t bad = s_bad[slot][0] | (uint64_t)s_bad[slot][1] << 32;
+    const uint64_t there = s_there[slot][0] | (uint64_t)s_there[slot][1] << 32;
+    if (key0 <= wlast) {
+      f32x16 s[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < G::NP; ++i) {
+          const uint4 a = *reinterpret_cast<const uint4*>(sk + lds_chunk<G::RB>(32 * n + col, 2 * i + half));
+          mma_chunk<T>(s[n], a, q[i]);
+        }
+      }
+      if (key0 + kKeyTile - 1 > wfirst || ~there != 0) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int i = 32 * n + key_of(r, half);
+            if (key0 + i > row.pos || !((there >> i) & 1)) s[n][r] = -INFINITY;
+          }
+      }
+      run.step(s, p.scale2);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) mma_values<T, D>(run.o, sk + kTileBytes, 32 * n, s[n], lane);
+      if (bad) add_nonfinite<T, D, 2>(run.o, s, bad, p, tile.n, kvh, key0, row.pos, lane);
+    }
+    if (t + 1 < tiles) stage(t + 1, next);
+    slot = next;
+    __syncthreads();
+  }
+  if (!row.live) return;
+  const float l = join_halves(run.l, [](float a, float b) { return a + b; });
+  if (tile.direct) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* dst = static_cast<T*>(p.o) + row.index * D;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        store4(dst + 32 * dt + key_of(r, half), make_float4(run.o[dt][r] * inv, run.o[dt][r + 1] * inv,
+                                                            run.o[dt][r + 2] * inv, run.o[dt][r + 3] * inv));
+    if (half == 0) p.lse[row.index] = (run.m + __log2f(l)) * 0.693147180559945309f;
+  } else {
+    const int64_t part = (int64_t)split * p.s.num_tokens * p.q_heads + row.index;
+    float* dst = p.part_o + part * D;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<float4*>(dst + 32 * dt + key_of(r, half)) =
+            make_float4(run.o[dt][r], run.o[dt][r + 1], run.o[dt][r + 2], run.o[dt][r + 3]);
+    if (half == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(run.m, l);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joining the splits of a row: one workgroup a row, its waves over the splits.
+// ---------------------------------------------------------------------------
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(AttnParams p) {
+  constexpr int L = D / 4;              // lanes of a part
+  constexpr int PP = kThreads / L;      // parts in flight
+  __shared__ float4 s_acc[kThreads];
+  __shared__ float s_sum[PP];
+  const int64_t rows = (int64_t)p.s.num_tokens * p.q_heads;
+  const int64_t row = blockIdx.x;
+  const int t = (int)(row / p.q_heads);
   const int n = seq_of_token(p.s, t);
   const SeqSpan span = seq_span(p.s, n);
   const int j = t - span.first;
-  const int last = n < p.s.num_seqs && (unsigned)j < (unsigned)span.count ? span.len - span.count + j : -1;
-  for (int c = lane; c < D; c += 64) s_q[w][c] = io<T>::load(static_cast<const T*>(p.q) + t * p.q_stride + (int64_t)h * D + c);
-  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-  constexpr int NC = D < 64 ? 1 : D / 64;
-  float acc[NC] = {}, m = -INFINITY, l = 0.f;
-  for (int p0 = 0; p0 <= last; p0 += 64) {
-    const int pos = p0 + lane;
-    int r = 0, page = -1;
-    if (pos <= last) page = page_of(p.s, n, pos, &r);
-    float s = -INFINITY;
-    const int64_t off = (int64_t)r * p.kv_heads * D + (int64_t)kvh * D;
-    if (page >= 0) {
-      const T* k = static_cast<const T*>(p.k_pages) + page * p.k_page_stride + off;
-      float x = 0.f;
-      for (int c = 0; c < D; ++c) x += s_q[w][c] * io<T>::load(k + c);
-      s = x * p.scale2;
-    }
-    float mx = s;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-    const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;
-    const float e = page >= 0 ? exp2_fast(s - base) : 0.f, a = exp2_fast(m - base);
-    m = mn;
-    float sum = e;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    l = l * a + sum;
-    s_p[w][lane] = e;
-    s_row[w][lane] = page >= 0 ? page * p.v_page_stride + off : -1;
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-#pragma unroll
-    for (int i = 0; i < NC; ++i) acc[i] *= a;
-    for (int i = 0; i < 64 && p0 + i <= last; ++i) {
-      const int64_t at = s_row[w][i];
-      if (at < 0) continue;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        if (lane < D) acc[c] += s_p[w][i] * io<T>::load(static_cast<const T*>(p.v_pages) + at + c * 64 + lane);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  if (n == p.s.num_seqs || (unsigned)j >= (unsigned)span.count) return;  // of no sequence: written already
+  const int chunk = split_chunk(span.len, p.splits);
+  if (span.len <= chunk) return;
+  const int pos = span.len - span.count + j;
+  const int parts = pos < 0 || p.s.num_pages == 0 ? 0 : pos / chunk + 1;
+  const int x = threadIdx.x / L, c = 4 * (threadIdx.x % L);
+  float m = -INFINITY;
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_ml[(i * rows + row) * 2]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int i = x; i < parts; i += PP) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (i * rows + row) * 2);
+    const float4 y = *reinterpret_cast<const float4*>(p.part_o + (i * rows + row) * D + c);
+    const float a = exp2_fast(ml.x - base);
+    sum += ml.y * a;
+    acc.x += y.x * a; acc.y += y.y * a; acc.z += y.z * a; acc.w += y.w * a;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-    if (lane < D) io<T>::store(static_cast<T*>(p.o) + row * D + c * 64 + lane, acc[c] * inv);
-  if (lane == 0) p.lse[row] = (m + __log2f(l)) * 0.693147180559945309f;
+  s_acc[threadIdx.x] = acc;
+  if (c == 0) s_sum[x] = sum;
+  __syncthreads();
+  if (x != 0) return;
+  for (int i = 1; i < PP; ++i) {
+    const float4 y = s_acc[i * L + threadIdx.x];
+    acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
+  }
+  sum = 0.f;
+  for (int i = 0; i < PP; ++i) sum += s_sum[i];
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  store4(static_cast<T*>(p.o) + row * D + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+  if (c == 0) p.lse[row] = (m + __log2f(sum)) * 0.693147180559945309f;
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+constexpr int64_t kTargetGroups = 512;  // two workgroups a compute unit
+
+// Splits of a sequence, at most: enough workgroups for the card where the tiles
+// alone are too few.
+int plan_splits(const AttnParams& p) {
+  const int64_t group = p.group.d, N = p.s.num_tokens, S = p.s.num_seqs;
+  const bool packed = p.s.cu != nullptr;
+  // sequences have N / S tokens each, by what the host knows
+  const bool rows_many = packed && N * group > 32 * S;
+  const int64_t tiles = rows_many ? tile_bound(N, S, group, kRowTile, true) : tile_bound(N, S, group, 32, packed);
+  const int64_t cap = ((int64_t)p.s.max_pages * p.s.page_size + kMinChunk - 1) / kMinChunk;
+  int64_t want = kTargetGroups / (tiles * p.kv_heads > 0 ? tiles * p.kv_heads : 1);
+  if (want > cap) want = cap;
+  if (want > 256) want = 256;
+  return want < 1 ? 1 : (int)want;
 }
 
 template <typename T, int D>
 int launch_attention(const AttnParams& p, hipStream_t s) {
-  const int64_t rows = (int64_t)p.s.num_tokens * p.q_heads;
-  const int64_t blocks = (rows + kThreads / 64 - 1) / (kThreads / 64);
-  PKDA_REQUIRE(blocks <= INT32_MAX, PKDA_EINVAL, "%lld rows", (long long)rows);
-  hipLaunchKernelGGL((paged_attention_rows_kernel<T, D>), dim3((unsigned)blocks), dim3(kThreads), 0, s, p);
-  return launch_status("pkda_paged_attention");
+  const bool packed = p.s.cu != nullptr;
+  const int64_t per_tile = (int64_t)p.kv_heads * p.splits;
+  const int64_t keys = tile_bound(p.s.num_tokens, p.s.num_seqs, p.group.d, 32, packed) * per_tile;
+  const int64_t rows = packed ? tile_bound(p.s.num_tokens, p.s.num_seqs, p.group.d, kRowTile, true) * per_tile : 0;
+  const int64_t join = (int64_t)p.s.num_tokens * p.q_heads;
+  PKDA_REQUIRE(keys <= INT32_MAX && rows <= INT32_MAX && join <= INT32_MAX, PKDA_EINVAL, "%d tokens of %d heads",
+               p.s.num_tokens, p.q_heads);
+  if (rows) {
+    hipLaunchKernelGGL((paged_attention_rows_kernel<T, D>), dim3((unsigned)rows), dim3(kThreads), 0, s, p);
+    if (int st = launch_status("pkda_paged_attention(rows)")) return st;
+  }
+  hipLaunchKernelGGL((paged_attention_keys_kernel<T, D>), dim3((unsigned)keys), dim3(kThreads), 0, s, p);
+  if (int st = launch_status("pkda_paged_attention(keys)")) return st;
+  if (p.splits > 1) {
+    hipLaunchKernelGGL((paged_attention_join_kernel<T, D>), dim3((unsigned)join), dim3(kThreads), 0, s, p);
+    return launch_status("pkda_paged_attention(join)");
+  }
+  return 0;
 }
 
 template <typename T>
@@ -106,7 +753,10 @@ int attention_sizes(const pkda_paged_attention_args* a, AttnParams& p) {
                "q_heads %d, kv_heads %d", a->q_heads, a->kv_heads);
   p.q_heads = a->q_heads;
   p.kv_heads = a->kv_heads;
-  p.group = a->q_heads / a->kv_heads;
+  p.group = FastDiv::make((uint32_t)(a->q_heads / a->kv_heads));
+  PKDA_REQUIRE((int64_t)a->num_tokens * p.group.d <= INT32_MAX, PKDA_EINVAL, "%d tokens of %d heads", a->num_tokens,
+               a->q_heads);
+  p.splits = plan_splits(p);
   return 0;
 }
 
@@ -116,7 +766,7 @@ int attention_sizes(const pkda_paged_attention_args* a, AttnParams& p) {
 extern "C" int64_t pkda_paged_attention_workspace(const pkda_paged_attention_args* a) {
   pkda::AttnParams p;
   if (pkda::attention_sizes(a, p)) return -1;
-  return 0;
+  return p.splits > 1 ? (int64_t)p.splits * a->num_tokens * a->q_heads * (a->head_dim + 2) : 0;
 }
 
 extern "C" int pkda_paged_attention(const pkda_paged_attention_args* a, void* stream) {
@@ -131,7 +781,14 @@ extern "C" int pkda_paged_attention(const pkda_paged_attention_args* a, void* st
                "q and o must be 16-byte aligned");
   p.q = a->q; p.q_stride = a->q_stride; p.k_pages = a->k_pages; p.v_pages = a->v_pages;
   p.k_page_stride = a->k_page_stride; p.v_page_stride = a->v_page_stride;
-  p.scale2 = a->scale * kLog2e;
+  PKDA_REQUIRE(isfinite(a->scale), PKDA_EINVAL, "scale %g", (double)a->scale);
+  // scale 0 as the smallest scale: a masked score stays -inf
+  p.negate = a->scale < 0.f;
+  p.scale2 = fmaxf(fabsf(a->scale) * kLog2e, 1e-37f);
+  const int64_t rows = (int64_t)a->num_tokens * a->q_heads;
+  PKDA_REQUIRE(p.splits == 1 || (a->workspace && (uintptr_t)a->workspace % 16 == 0), PKDA_EINVAL, "workspace");
+  p.part_o = a->workspace;
+  p.part_ml = a->workspace ? a->workspace + p.splits * rows * a->head_dim : nullptr;
   p.o = a->o; p.lse = a->lse;
   hipStream_t s = static_cast<hipStream_t>(stream);
   return a->dtype == PKDA_BF16 ? attention_dim<bf16_t>(p, a->head_dim, s) : attention_dim<float>(p, a->head_dim, s);
