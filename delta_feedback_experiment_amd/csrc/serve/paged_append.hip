@@ -106,7 +106,10 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendParams p) 
   const int pos = span.len - span.count + (t - span.first);
   const bool placed = n < p.s.num_seqs && (unsigned)(t - span.first) < (unsigned)span.count && pos >= 0;
   int row = 0, page = -1;
-  if (placed) page = page_of(p.s, n, pos, &row);
+  if (placed) {
+    page = page_entry(p.s, n, pos, &row);
+    if (!page_exists(p.s, page)) page = -1;
+  }
 
   float cs[8], sn[8];
   if (turns && placed) {

@@ -36,6 +36,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMinChunk = 128;  // keys of a split, at least
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -83,7 +84,7 @@ __device__ __forceinline__ int lds_chunk(int row, int chunk) {  // byte offset
 
 // acc += A B over one chunk pair; lane: row / column lane & 31, the half's chunk.
 template <typename T>
-__device__ __forceinline__ void mma_chunk(f32x16& acc, const uint4& a, const uint4& b) {
+__device__ __forceinline__ void mma_chunk(f32x16& acc, const u32x4& a, const u32x4& b) {
   if constexpr (sizeof(T) == 2) {
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
   } else {
@@ -139,7 +140,7 @@ __device__ __forceinline__ float join_halves(float x, F f) {
 
 // The numbers of a chunk that are not finite become zero; whether there were any.
 template <typename T>
-__device__ __forceinline__ bool clear_nonfinite(uint4& x) {
+__device__ __forceinline__ bool clear_nonfinite(u32x4& x) {
   uint32_t w[4] = {x.x, x.y, x.z, x.w};
   bool any = false;
 #pragma unroll
@@ -151,7 +152,7 @@ __device__ __forceinline__ bool clear_nonfinite(uint4& x) {
       if ((w[i] & 0x7f800000u) == 0x7f800000u) { any = true; w[i] = 0; }
     }
   }
-  x = make_uint4(w[0], w[1], w[2], w[3]);
+  x = u32x4{w[0], w[1], w[2], w[3]};
   return any;
 }
 
@@ -213,14 +214,14 @@ struct Row {
 };
 template <typename T, int D>
 __device__ __forceinline__ Row load_row(const AttnParams& p, const Tile& tile, int kvh, int r, int half,
-                                        uint4 (&q)[Geo<T, D>::NP]) {
+                                        u32x4 (&q)[Geo<T, D>::NP]) {
   using G = Geo<T, D>;
   Row row;
   row.live = r < tile.rows;
   row.pos = -1;
   row.index = 0;
 #pragma unroll
-  for (int i = 0; i < G::NP; ++i) q[i] = make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < G::NP; ++i) q[i] = u32x4{0, 0, 0, 0};
   if (row.live) {
     const int j = (int)p.group.div((uint32_t)r), g = r - j * (int)p.group.d;
     const int h = kvh * (int)p.group.d + g, t = tile.span.first + j;
@@ -228,13 +229,17 @@ __device__ __forceinline__ Row load_row(const AttnParams& p, const Tile& tile, i
     row.pos = max(-1, tile.span.len - tile.span.count + j);
     const T* src = static_cast<const T*>(p.q) + t * p.q_stride + (int64_t)h * D + half * G::EC;
 #pragma unroll
-    for (int i = 0; i < G::NP; ++i) q[i] = *reinterpret_cast<const uint4*>(src + 2 * i * G::EC);
+    for (int i = 0; i < G::NP; ++i) q[i] = *reinterpret_cast<const u32x4*>(src + 2 * i * G::EC);
     if (p.negate) {
       const uint32_t sign = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
 #pragma unroll
-      for (int i = 0; i < G::NP; ++i) { q[i].x ^= sign; q[i].y ^= sign; q[i].z ^= sign; q[i].w ^= sign; }
+      for (int i = 0; i < G::NP; ++i) q[i] ^= sign;
     }
   }
+  // the queries arrive before the loop over the keys: waits inside it would hold
+  // the keys that are on their way
+#pragma unroll
+  for (int i = 0; i < G::NP; ++i) asm volatile("" : "+v"(q[i]));
   return row;
 }
 
@@ -296,8 +301,8 @@ __device__ __forceinline__ void add_nonfinite(f32x16 (&o)[D / 32], const f32x16 
     const int i = __builtin_ctzll(bad);
     bad &= bad - 1;
     int row;
-    const int page = page_of(p.s, n, key0 + i, &row);
-    if (page < 0) continue;
+    const int page = page_entry(p.s, n, key0 + i, &row);
+    if (!page_exists(p.s, page)) continue;
     const T* v = static_cast<const T*>(p.v_pages) + page * p.v_page_stride + ((int64_t)row * p.kv_heads + kvh) * D;
     const int key_half = (i >> 2) & 1, key_r = 4 * ((i & 31) >> 3) + (i & 3);
     float pr = 0.f;  // the key's probability, in the lanes of its half
@@ -349,7 +354,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) voi
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 31, half = lane >> 5;
-  uint4 q[G::NP];
+  u32x4 q[G::NP];
   const Row row = load_row<T, D>(p, tile, kvh, tile.row0 + col, half, q);
   Running<G::DT> run;
   run.init();
@@ -360,32 +365,35 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) voi
   const T* vb = static_cast<const T*>(p.v_pages) + (int64_t)kvh * D + half * G::EC;
   const int row_stride = p.kv_heads * D;
 
-  // page and row of this lane's key of tile t
-  const auto look = [&](int t, int& r) -> int {
-    const int key = k0 + 32 * t + col;
-    const int page = page_of(p.s, tile.n, min(key, k1 - 1), &r);
-    return key < k1 ? page : -1;
-  };
-  uint4 k[G::NP], v[G::NP];
-  const auto load = [&](int page, int r) {
-    const int64_t at = page < 0 ? 0 : page, off = page < 0 ? 0 : (int64_t)r * row_stride;
+  // the table's entry and the row of this lane's key of tile t: looked up a
+  // tile ahead and read only where the keys are loaded, so that nothing waits
+  const auto look = [&](int t, int& r) -> int { return page_entry(p.s, tile.n, min(k0 + 32 * t + col, k1 - 1), &r); };
+  u32x4 k[G::NP], v[G::NP];
+  bool here = false;  // this lane's key is there
+  const auto load = [&](int t, int page, int r) {
+    here = page_exists(p.s, page);
+    const int64_t at = here ? page : 0, off = here ? (int64_t)r * row_stride : 0;
+    here = here && k0 + 32 * t + col < k1;
     const T* ks = kb + at * p.k_page_stride + off;
     const T* vs = vb + at * p.v_page_stride + off;
 #pragma unroll
-    for (int i = 0; i < G::NP; ++i) k[i] = *reinterpret_cast<const uint4*>(ks + 2 * i * G::EC);
+    for (int i = 0; i < G::NP; ++i) k[i] = *reinterpret_cast<const u32x4*>(ks + 2 * i * G::EC);
 #pragma unroll
-    for (int i = 0; i < G::NP; ++i) v[i] = *reinterpret_cast<const uint4*>(vs + 2 * i * G::EC);
+    for (int i = 0; i < G::NP; ++i) v[i] = *reinterpret_cast<const u32x4*>(vs + 2 * i * G::EC);
   };
 
-  int page = -1, page1 = -1, r0 = 0, r1 = 0;
+  int page = 0, r = 0;
   if (w < tiles) {
-    page = look(w, r0);
+    page = look(w, r);
+    int page1 = 0, r1 = 0;
     if (w + kWaves < tiles) page1 = look(w + kWaves, r1);
-    load(page, r0);
+    load(w, page, r);
+    page = page1;
+    r = r1;
   }
   for (int t = w; t < tiles; t += kWaves) {
     const int key0 = k0 + 32 * t;
-    const uint32_t there = (uint32_t)__ballot(page >= 0);
+    const uint32_t there = (uint32_t)__ballot(here);
     f32x16 s[1];
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
@@ -396,9 +404,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) voi
     const bool partial = key0 + 31 > tile.first;
     uint32_t bad = 0;
     if (there != 0xffffffffu) {
-      if (page < 0)
+      if (!here)
 #pragma unroll
-        for (int i = 0; i < G::NP; ++i) v[i] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < G::NP; ++i) v[i] = u32x4{0, 0, 0, 0};
     }
     if (partial && tile.first != tile.last) {
       bool any = false;
@@ -408,11 +416,13 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) voi
       bad = (uint32_t)b | (uint32_t)(b >> 32);
     }
 #pragma unroll
-    for (int i = 0; i < G::NP; ++i) *reinterpret_cast<uint4*>(sv + lds_chunk<G::RB>(col, 2 * i + half)) = v[i];
-    page = page1;
+    for (int i = 0; i < G::NP; ++i) *reinterpret_cast<u32x4*>(sv + lds_chunk<G::RB>(col, 2 * i + half)) = v[i];
     if (t + kWaves < tiles) {
-      load(page1, r1);
+      int page1 = 0, r1 = 0;
       if (t + 2 * kWaves < tiles) page1 = look(t + 2 * kWaves, r1);
+      load(t + kWaves, page, r);
+      page = page1;
+      r = r1;
     }
     if (partial || there != 0xffffffffu) {
 #pragma unroll
@@ -485,15 +495,19 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) voi
 constexpr int kRowTile = 32 * kWaves;
 constexpr int kKeyTile = 64;
 
-template <typename T, int D>
+// WHOLE: the rows that a wave stages at a time, 64 / NC keys, lie in one page
+// (the page size is a multiple of them): their page is looked up once a wave,
+// in scalar registers, and a lane's address is that plus a constant.
+template <typename T, int D, bool WHOLE>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) void paged_attention_rows_kernel(AttnParams p) {
   using G = Geo<T, D>;
   constexpr int NI = kKeyTile * G::NC / kThreads;  // chunks of K (and of V) a thread stages
   constexpr int RI = kThreads / G::NC;             // rows a pass of the workgroup covers
+  constexpr int RW = 64 / G::NC;                   // and a wave of it
   constexpr int kTileBytes = kKeyTile * G::RB;
   __shared__ __align__(16) char s_kv[4 * kTileBytes];  // two stages of K, V
-  __shared__ uint32_t s_bad[3][2];    // tile t % 3: its keys with values that are not finite
-  __shared__ uint32_t s_there[3][2];  // and those that have a page
+  // of tile t % 3: its keys with values that are not finite, and those without a page
+  __shared__ __align__(16) uint32_t s_odd[3][4];
 
   const int kvh = blockIdx.x % p.kv_heads;
   const int rest = blockIdx.x / p.kv_heads;
@@ -507,7 +521,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) voi
 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int col = lane & 31, half = lane >> 5;
-  uint4 q[G::NP];
+  u32x4 q[G::NP];
   const int wrow0 = tile.row0 + 32 * w;
   const Row row = load_row<T, D>(p, tile, kvh, wrow0 + col, half, q);
   // positions of the wave's first and last live row
@@ -528,71 +542,83 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) voi
   const auto look = [&](int t) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int key = k0 + kKeyTile * t + RI * i + srow;
-      const int at = page_of(p.s, tile.n, min(key, k1 - 1), &prow[i]);
-      page[i] = key < k1 ? at : -1;
+      if constexpr (WHOLE) {
+        const int key = min(k0 + kKeyTile * t + RI * i + RW * w, (k1 - 1) / RW * RW);
+        page[i] = page_entry(p.s, tile.n, key, &prow[i]);
+      } else {
+        const int key = k0 + kKeyTile * t + RI * i + srow;
+        page[i] = page_entry(p.s, tile.n, min(key, k1 - 1), &prow[i]);
+      }
     }
   };
-  uint4 k[NI], v[NI];
-  uint32_t held;  // this thread's staged rows that are there, one bit each
-  const auto load = [&]() {
-    held = 0;
+  const int lane_off = WHOLE ? (srow - RW * w) * row_stride : 0;
+  u32x4 k[NI], v[NI];
+  uint32_t gone = 0;  // this thread's staged rows that are not there, one bit each
+  const auto load = [&](int t) {
+    const T *ks[NI], *vs[NI];
+    gone = 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int64_t at = page[i] < 0 ? 0 : page[i], off = page[i] < 0 ? 0 : (int64_t)prow[i] * row_stride;
-      held |= (page[i] < 0 ? 0u : 1u) << i;
-      k[i] = *reinterpret_cast<const uint4*>(kb + at * p.k_page_stride + off);
-      v[i] = *reinterpret_cast<const uint4*>(vb + at * p.v_page_stride + off);
+      int at = page[i], r = prow[i];
+      if constexpr (WHOLE) at = __builtin_amdgcn_readfirstlane(at);
+      if (!page_exists(p.s, at)) {
+        gone |= 1u << i;
+        at = r = 0;
+      }
+      ks[i] = kb + at * p.k_page_stride + (int64_t)r * row_stride;
+      vs[i] = vb + at * p.v_page_stride + (int64_t)r * row_stride;
+    }
+    if (t + 1 < tiles) look(t + 1);  // before the keys' loads, which it would otherwise wait for
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      k[i] = *reinterpret_cast<const u32x4*>(ks[i] + lane_off);
+      v[i] = *reinterpret_cast<const u32x4*>(vs[i] + lane_off);
+    }
+    if (k0 + kKeyTile * (t + 1) > k1) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) gone |= (k0 + kKeyTile * t + srow + RI * i < k1 ? 0u : 1u) << i;
     }
   };
   const auto stage = [&](int t, int slot) {
     char* sk = s_kv + (t & 1) * 2 * kTileBytes;
-    const bool check = k0 + kKeyTile * t + kKeyTile - 1 > tile.first;
-    uint32_t bad = 0;
-    if (held != (1u << NI) - 1u) {
+    if (__any(gone)) {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
-        if (!((held >> i) & 1)) v[i] = make_uint4(0, 0, 0, 0);
+        if ((gone >> i) & 1) {
+          const int r = RI * i + srow;
+          v[i] = u32x4{0, 0, 0, 0};
+          if (schunk == 0) atomicOr(&s_odd[slot][2 + (r >> 5)], 1u << (r & 31));
+        }
     }
-    if (check) {
+    if (k0 + kKeyTile * t + kKeyTile - 1 > tile.first) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) bad |= (clear_nonfinite<T>(v[i]) ? 1u : 0u) << i;
+      for (int i = 0; i < NI; ++i) {
+        const int r = RI * i + srow;
+        if (clear_nonfinite<T>(v[i])) atomicOr(&s_odd[slot][r >> 5], 1u << (r & 31));
+      }
     }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int r = RI * i + srow, at = lds_chunk<G::RB>(r, schunk);
-      *reinterpret_cast<uint4*>(sk + at) = k[i];
-      *reinterpret_cast<uint4*>(sk + kTileBytes + at) = v[i];
-      if ((bad >> i) & 1) atomicOr(&s_bad[slot][r >> 5], 1u << (r & 31));
-      if (!((held >> i) & 1) && schunk == 0) atomicAnd(&s_there[slot][r >> 5], ~(1u << (r & 31)));
+      const int at = lds_chunk<G::RB>(RI * i + srow, schunk);
+      *reinterpret_cast<u32x4*>(sk + at) = k[i];
+      *reinterpret_cast<u32x4*>(sk + kTileBytes + at) = v[i];
     }
   };
-  if (tid < 6) {
-    s_bad[tid >> 1][tid & 1] = 0;
-    s_there[tid >> 1][tid & 1] = 0xffffffffu;
-  }
+  if (tid < 12) s_odd[tid >> 2][tid & 3] = 0;
   __syncthreads();
   if (tiles > 0) {
     look(0);
-    load();
-    if (tiles > 1) look(1);
+    load(0);
     stage(0, 0);
   }
   __syncthreads();
   int slot = 0;
   for (int t = 0; t < tiles; ++t) {
     const int key0 = k0 + kKeyTile * t, next = slot == 2 ? 0 : slot + 1, free = next == 2 ? 0 : next + 1;
-    if (tid < 2) {  // tile t + 2's, read last before the barrier that ended tile t - 1
-      s_bad[free][tid] = 0;
-      s_there[free][tid] = 0xffffffffu;
-    }
-    if (t + 1 < tiles) {
-      load();
-      if (t + 2 < tiles) look(t + 2);
-    }
+    if (tid < 4) s_odd[free][tid] = 0;  // tile t + 2's, read last before the barrier that ended tile t - 1
+    if (t + 1 < tiles) load(t + 1);
     const char* sk = s_kv + (t & 1) * 2 * kTileBytes;
-    const uint64_t bad = s_bad[slot][0] | (uint64_t)s_bad[slot][1] << 32;
-    const uint64_t there = s_there[slot][0] | (uint64_t)s_there[slot][1] << 32;
+    const u32x4 odd = *reinterpret_cast<const u32x4*>(s_odd[slot]);
     if (key0 <= wlast) {
       f32x16 s[2];
 #pragma unroll
@@ -601,22 +627,31 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) voi
         for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
 #pragma unroll
         for (int i = 0; i < G::NP; ++i) {
-          const uint4 a = *reinterpret_cast<const uint4*>(sk + lds_chunk<G::RB>(32 * n + col, 2 * i + half));
+          const u32x4 a = *reinterpret_cast<const u32x4*>(sk + lds_chunk<G::RB>(32 * n + col, 2 * i + half));
           mma_chunk<T>(s[n], a, q[i]);
         }
       }
-      if (key0 + kKeyTile - 1 > wfirst || ~there != 0) {
+      const uint32_t gone0 = __builtin_amdgcn_readfirstlane(odd.z), gone1 = __builtin_amdgcn_readfirstlane(odd.w);
+      if (key0 + kKeyTile - 1 > wfirst) {
+        const int sees = row.pos - key0;  // the row sees keys up to this one of the tile
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int i = 32 * n + key_of(r, half);
-            if (key0 + i > row.pos || !((there >> i) & 1)) s[n][r] = -INFINITY;
-          }
+          for (int r = 0; r < 16; ++r)
+            if (32 * n + key_of(r, half) > sees) s[n][r] = -INFINITY;
+      }
+      if (gone0 | gone1) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (((n ? gone1 : gone0) >> key_of(r, half)) & 1) s[n][r] = -INFINITY;
       }
       run.step(s, p.scale2);
 #pragma unroll
       for (int n = 0; n < 2; ++n) mma_values<T, D>(run.o, sk + kTileBytes, 32 * n, s[n], lane);
+      const uint64_t bad = __builtin_amdgcn_readfirstlane(odd.x) |
+                           (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(odd.y) << 32;
       if (bad) add_nonfinite<T, D, 2>(run.o, s, bad, p, tile.n, kvh, key0, row.pos, lane);
     }
     if (t + 1 < tiles) stage(t + 1, next);
@@ -726,7 +761,10 @@ int launch_attention(const AttnParams& p, hipStream_t s) {
   PKDA_REQUIRE(keys <= INT32_MAX && rows <= INT32_MAX && join <= INT32_MAX, PKDA_EINVAL, "%d tokens of %d heads",
                p.s.num_tokens, p.q_heads);
   if (rows) {
-    hipLaunchKernelGGL((paged_attention_rows_kernel<T, D>), dim3((unsigned)rows), dim3(kThreads), 0, s, p);
+    if (p.s.page_size % (64 / Geo<T, D>::NC) == 0)
+      hipLaunchKernelGGL((paged_attention_rows_kernel<T, D, true>), dim3((unsigned)rows), dim3(kThreads), 0, s, p);
+    else
+      hipLaunchKernelGGL((paged_attention_rows_kernel<T, D, false>), dim3((unsigned)rows), dim3(kThreads), 0, s, p);
     if (int st = launch_status("pkda_paged_attention(rows)")) return st;
   }
   hipLaunchKernelGGL((paged_attention_keys_kernel<T, D>), dim3((unsigned)keys), dim3(kThreads), 0, s, p);

@@ -31,7 +31,7 @@ struct PagedSeqs {
   const int32_t* lens;
   const int32_t* table;
   int64_t table_stride;
-  int64_t num_pages;
+  int num_pages;
   int num_seqs, num_tokens;
   int page_size, max_pages;
   FastDiv page;
@@ -90,13 +90,16 @@ __device__ __forceinline__ int seq_of_token(const PagedSeqs& s, int t) {
   });
 }
 
-// The page of position p of sequence n, or -1 when the table names none in
-// the pool (0 <= p < max_pages * page_size).
-__device__ __forceinline__ int page_of(const PagedSeqs& s, int n, int p, int* row) {
+// What the table says of position p of sequence n (0 <= p < max_pages *
+// page_size), and the position's row of that page.
+__device__ __forceinline__ int page_entry(const PagedSeqs& s, int n, int p, int* row) {
   const int i = (int)s.page.div((uint32_t)p);
   *row = p - i * s.page_size;
-  const int page = s.table[(int64_t)n * s.table_stride + i];
-  return page >= 0 && page < s.num_pages ? page : -1;
+  return s.table[(int64_t)n * s.table_stride + i];
+}
+// Whether the pool has such a page.
+__device__ __forceinline__ bool page_exists(const PagedSeqs& s, int page) {
+  return (uint32_t)page < (uint32_t)s.num_pages;
 }
 
 // Host: the arguments that append and attention share.
@@ -112,7 +115,7 @@ int paged_seqs_from(const A* a, PagedSeqs& s) {
                PKDA_EINVAL, "page_size %d x %d pages of a table row", a->page_size, a->max_pages);
   PKDA_REQUIRE(a->num_pages >= 0 && a->num_pages <= INT32_MAX, PKDA_EINVAL, "num_pages");
   s.cu = a->cu_seqlens; s.lens = a->seq_lens; s.table = a->page_table;
-  s.table_stride = a->table_stride; s.num_pages = a->num_pages;
+  s.table_stride = a->table_stride; s.num_pages = (int)a->num_pages;
   s.num_seqs = a->num_seqs; s.num_tokens = a->num_tokens;
   s.page_size = a->page_size; s.max_pages = a->max_pages;
   s.page = FastDiv::make((uint32_t)a->page_size);
