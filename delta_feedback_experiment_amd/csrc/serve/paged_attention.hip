@@ -18,13 +18,13 @@
 // half of a row is operand i of the lane's half (BF16: one 32x32x16 step; FP32:
 // four 32x32x2 steps).
 //
-// Two kernels.  Up to 32 rows of a tile (decode): four waves take 32 keys each
+// Two forms, in one launch.  Up to 32 rows of a tile (decode): four waves take 32 keys each
 // in turn, each with its own m, l and O, and join at the end; keys go straight
 // from memory to operand registers, values through a wave's own piece of LDS
 // (the transposing reads), the next tile's loads in flight during a tile's
 // arithmetic.  More rows (a chunk): four waves of 32 rows share tiles of 64 keys
 // staged in LDS, double-buffered.  Where rows are few, a sequence's keys are
-// split over workgroups and a third kernel joins the parts.
+// split over workgroups and a second kernel joins the parts.
 #include <math.h>
 
 #include "paged_common.h"
@@ -34,7 +34,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMinChunk = 128;  // keys of a split, at least
+constexpr int kMaxSplits = 256;
+constexpr int kMinChunk = 128;  // a split is a multiple of so many keys
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -54,6 +55,9 @@ struct AttnParams {
   float scale2;  // |scale| log2 e: the softmax is taken in base 2
   bool negate;   // scale < 0: queries are negated
   int splits;
+  int min_chunk;       // keys of a split, at least
+  int key_rows;        // sequences of up to so many rows run with their keys over the waves
+  unsigned row_blocks; // workgroups of the others, before those
   void* o;
   float* lse;
   float* part_o;   // [splits][num_tokens * q_heads][head_dim]
@@ -166,9 +170,9 @@ struct Tile {
   bool direct;        // the sequence is not split: this workgroup has the whole softmax
 };
 
-__device__ __forceinline__ int split_chunk(int len, int splits) {
-  const int c = (len + splits - 1) / splits;
-  return max(kMinChunk, (c + kMinChunk - 1) / kMinChunk * kMinChunk);
+__device__ __forceinline__ int split_chunk(const AttnParams& p, int len) {
+  const int c = (len + p.splits - 1) / p.splits;
+  return max(p.min_chunk, (c + kMinChunk - 1) / kMinChunk * kMinChunk);
 }
 
 // Tiles are numbered through the sequences with room for one that is not full
@@ -181,7 +185,10 @@ template <int M>
 __device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& tile) {
   const int group = (int)p.group.d;
   int local;
-  if (p.s.cu) {
+  if (M == 32 && p.s.cu && p.key_rows == 32) {  // one tile a sequence
+    tile.n = (int)t;
+    local = 0;
+  } else if (p.s.cu) {
     const auto begin = [&](int n) -> int64_t {
       return (n == 0 ? 0 : (int64_t)clamp_int(p.s.cu[n], 0, p.s.num_tokens) * group / M) + n;
     };
@@ -201,7 +208,7 @@ __device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& 
   tile.first = base + (int)p.group.div((uint32_t)row0);
   tile.last = base + (int)p.group.div((uint32_t)min(rows - 1, row0 + M - 1));
   tile.keys = p.s.num_pages == 0 ? 0 : max(0, tile.last + 1);
-  tile.chunk = split_chunk(tile.span.len, p.splits);
+  tile.chunk = split_chunk(p, tile.span.len);
   tile.direct = tile.span.len <= tile.chunk;
   return true;
 }
@@ -335,20 +342,27 @@ __device__ __forceinline__ void add_nonfinite(f32x16 (&o)[D / 32], const f32x16 
 // ---------------------------------------------------------------------------
 // Up to 32 rows a tile: the keys over the waves.
 // ---------------------------------------------------------------------------
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) void paged_attention_keys_kernel(AttnParams p) {
-  using G = Geo<T, D>;
-  constexpr int OS = D + 4;  // floats between the rows of a wave's output in LDS
-  constexpr int kStage = kWaves * 32 * G::RB, kJoin = kWaves * 32 * OS * 4;
-  __shared__ __align__(16) char s_buf[kStage > kJoin ? kStage : kJoin];
-  __shared__ float s_m[kWaves][32], s_l[kWaves][32];
+template <typename T, int D> struct KeysLds {
+  static constexpr int OS = D + 4;  // floats between the rows of a wave's output
+  static constexpr int kStage = kWaves * 32 * Geo<T, D>::RB, kJoin = kWaves * 32 * OS * 4;
+  __align__(16) char buf[kStage > kJoin ? kStage : kJoin];
+  float m[kWaves][32], l[kWaves][32];
+};
 
-  const int kvh = blockIdx.x % p.kv_heads;
-  const int rest = blockIdx.x / p.kv_heads;
+template <typename T, int D>
+__device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block, KeysLds<T, D>& lds) {
+  using G = Geo<T, D>;
+  constexpr int OS = KeysLds<T, D>::OS;
+  char* s_buf = lds.buf;
+  float (&s_m)[kWaves][32] = lds.m;
+  float (&s_l)[kWaves][32] = lds.l;
+
+  const int kvh = block % p.kv_heads;
+  const unsigned rest = block / p.kv_heads;
   const int split = rest % p.splits;
   Tile tile;
   if (!find_tile<32>(p, rest / p.splits, tile)) return;
-  if (p.s.cu && (int64_t)tile.rows > 32) return;  // the other kernel's
+  if (p.s.cu && tile.rows > p.key_rows) return;  // the other form's
   const int k0 = split * tile.chunk, k1 = min(k0 + tile.chunk, tile.keys);
   if (split > 0 && (k0 >= tile.keys || tile.direct)) return;
 
@@ -498,24 +512,29 @@ constexpr int kKeyTile = 64;
 // WHOLE: the rows that a wave stages at a time, 64 / NC keys, lie in one page
 // (the page size is a multiple of them): their page is looked up once a wave,
 // in scalar registers, and a lane's address is that plus a constant.
+template <typename T, int D> struct RowsLds {
+  __align__(16) char kv[4 * kKeyTile * Geo<T, D>::RB];  // two stages of K, V
+  // of tile t % 3: its keys with values that are not finite, and those without a page
+  __align__(16) uint32_t odd[3][4];
+};
+
 template <typename T, int D, bool WHOLE>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) void paged_attention_rows_kernel(AttnParams p) {
+__device__ __forceinline__ void attend_rows(const AttnParams& p, unsigned block, RowsLds<T, D>& lds) {
   using G = Geo<T, D>;
   constexpr int NI = kKeyTile * G::NC / kThreads;  // chunks of K (and of V) a thread stages
   constexpr int RI = kThreads / G::NC;             // rows a pass of the workgroup covers
   constexpr int RW = 64 / G::NC;                   // and a wave of it
   constexpr int kTileBytes = kKeyTile * G::RB;
-  __shared__ __align__(16) char s_kv[4 * kTileBytes];  // two stages of K, V
-  // of tile t % 3: its keys with values that are not finite, and those without a page
-  __shared__ __align__(16) uint32_t s_odd[3][4];
+  char* s_kv = lds.kv;
+  uint32_t (&s_odd)[3][4] = lds.odd;
 
-  const int kvh = blockIdx.x % p.kv_heads;
-  const int rest = blockIdx.x / p.kv_heads;
+  const int kvh = block % p.kv_heads;
+  const unsigned rest = block / p.kv_heads;
   const int split = rest % p.splits;
   const int64_t bound = tile_bound(p.s.num_tokens, p.s.num_seqs, p.group.d, kRowTile, true);
   Tile tile;
   if (!find_tile<kRowTile>(p, bound - 1 - rest / p.splits, tile)) return;  // the longest first
-  if ((int64_t)tile.rows <= 32) return;                                    // the other kernel's
+  if (tile.rows <= p.key_rows) return;                                     // the other form's
   const int k0 = split * tile.chunk, k1 = min(k0 + tile.chunk, tile.keys);
   if (split > 0 && (k0 >= tile.keys || tile.direct)) return;
 
@@ -684,48 +703,78 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) voi
 }
 
 // ---------------------------------------------------------------------------
-// Joining the splits of a row: one workgroup a row, its waves over the splits.
-// ---------------------------------------------------------------------------
+template <typename T, int D, bool WHOLE>
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) void paged_attention_kernel(AttnParams p) {
+  __shared__ union Lds {
+    KeysLds<T, D> keys;
+    RowsLds<T, D> rows;
+  } lds;
+  if (blockIdx.x < p.row_blocks) attend_rows<T, D, WHOLE>(p, blockIdx.x, lds.rows);
+  else attend_keys<T, D>(p, blockIdx.x - p.row_blocks, lds.keys);
+}
+// Without cu_seqlens every sequence has group rows and only the first form runs.
 template <typename T, int D>
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2) void paged_attention_token_kernel(AttnParams p) {
+  __shared__ KeysLds<T, D> lds;
+  attend_keys<T, D>(p, blockIdx.x, lds);
+}
+
+// ---------------------------------------------------------------------------
+// Joining the splits of a row: W waves a row, lanes over channels and parts.
+// ---------------------------------------------------------------------------
+template <typename T, int D, int W>
 __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(AttnParams p) {
-  constexpr int L = D / 4;              // lanes of a part
-  constexpr int PP = kThreads / L;      // parts in flight
+  constexpr int N = 64 * W;     // threads of a row
+  constexpr int L = D / 4;      // threads of a part
+  constexpr int PP = N / L;     // parts at a time
+  constexpr int R = kThreads / N;
   __shared__ float4 s_acc[kThreads];
-  __shared__ float s_sum[PP];
+  __shared__ float s_w[R][kMaxSplits];
   const int64_t rows = (int64_t)p.s.num_tokens * p.q_heads;
-  const int64_t row = blockIdx.x;
-  const int t = (int)(row / p.q_heads);
+  const int slot = W == kWaves ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / N);
+  const int tid = threadIdx.x % N, lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * R + slot;
+  bool mine = row < rows;
+  const int t = mine ? (int)(row / p.q_heads) : 0;
   const int n = seq_of_token(p.s, t);
   const SeqSpan span = seq_span(p.s, n);
   const int j = t - span.first;
-  if (n == p.s.num_seqs || (unsigned)j >= (unsigned)span.count) return;  // of no sequence: written already
-  const int chunk = split_chunk(span.len, p.splits);
-  if (span.len <= chunk) return;
+  const int chunk = split_chunk(p, span.len);
+  // written already: rows of no sequence, and those of one that is not split
+  mine = mine && n < p.s.num_seqs && (unsigned)j < (unsigned)span.count && span.len > chunk;
   const int pos = span.len - span.count + j;
-  const int parts = pos < 0 || p.s.num_pages == 0 ? 0 : pos / chunk + 1;
-  const int x = threadIdx.x / L, c = 4 * (threadIdx.x % L);
+  const int parts = !mine || pos < 0 || p.s.num_pages == 0 ? 0 : pos / chunk + 1;
+  // every wave finds the row's maximum and sum for itself
   float m = -INFINITY;
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_ml[(i * rows + row) * 2]);
+  for (int i = lane; i < parts; i += 64) m = fmaxf(m, p.part_ml[(i * rows + row) * 2]);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   const float base = m == -INFINITY ? 0.f : m;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
-  for (int i = x; i < parts; i += PP) {
+  for (int i = lane; i < parts; i += 64) {
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (i * rows + row) * 2);
-    const float4 y = *reinterpret_cast<const float4*>(p.part_o + (i * rows + row) * D + c);
     const float a = exp2_fast(ml.x - base);
     sum += ml.y * a;
+    if (tid < 64) s_w[slot][i] = a;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  __syncthreads();
+  const int x = tid / L, c = 4 * (tid % L);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = x; i < parts; i += PP) {
+    const float4 y = *reinterpret_cast<const float4*>(p.part_o + (i * rows + row) * D + c);
+    const float a = s_w[slot][i];
     acc.x += y.x * a; acc.y += y.y * a; acc.z += y.z * a; acc.w += y.w * a;
   }
   s_acc[threadIdx.x] = acc;
-  if (c == 0) s_sum[x] = sum;
   __syncthreads();
-  if (x != 0) return;
+  if (x != 0 || !mine) return;
   for (int i = 1; i < PP; ++i) {
-    const float4 y = s_acc[i * L + threadIdx.x];
+    const float4 y = s_acc[threadIdx.x + i * L];
     acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
   }
-  sum = 0.f;
-  for (int i = 0; i < PP; ++i) sum += s_sum[i];
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   store4(static_cast<T*>(p.o) + row * D + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   if (c == 0) p.lse[row] = (m + __log2f(sum)) * 0.693147180559945309f;
@@ -734,46 +783,62 @@ __global__ __launch_bounds__(kThreads) void paged_attention_join_kernel(AttnPara
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-constexpr int64_t kTargetGroups = 512;  // two workgroups a compute unit
+constexpr int64_t kSlots = 512;  // workgroups the card holds: two a compute unit
 
-// Splits of a sequence, at most: enough workgroups for the card where the tiles
-// alone are too few.
-int plan_splits(const AttnParams& p) {
-  const int64_t group = p.group.d, N = p.s.num_tokens, S = p.s.num_seqs;
+struct Plan {
+  int64_t row_tiles, key_tiles;
+};
+
+// Which form takes which sequences, and into how many splits a sequence's keys
+// are cut at most, from what the host knows: sequences have num_tokens /
+// num_seqs tokens each.
+Plan plan(AttnParams& p) {
+  const int64_t group = p.group.d, N = p.s.num_tokens, S = p.s.num_seqs, heads = p.kv_heads;
   const bool packed = p.s.cu != nullptr;
-  // sequences have N / S tokens each, by what the host knows
-  const bool rows_many = packed && N * group > 32 * S;
-  const int64_t tiles = rows_many ? tile_bound(N, S, group, kRowTile, true) : tile_bound(N, S, group, 32, packed);
-  const int64_t cap = ((int64_t)p.s.max_pages * p.s.page_size + kMinChunk - 1) / kMinChunk;
-  int64_t want = kTargetGroups / (tiles * p.kv_heads > 0 ? tiles * p.kv_heads : 1);
+  Plan r;
+  p.key_rows = 32;
+  r.row_tiles = packed ? tile_bound(N, S, group, kRowTile, true) : 0;
+  if (packed && r.row_tiles * heads < kSlots / 2) p.key_rows = INT32_MAX;
+  if (p.key_rows != 32) r.row_tiles = 0;
+  r.key_tiles = packed && p.key_rows == 32 ? S + 1 : tile_bound(N, S, group, 32, packed);
+  // a row's part of a split costs 2 D floats, a key 2 D numbers a tile: enough
+  // keys a split that the parts stay a small share
+  const int64_t per_seq = S > 0 ? (N * group + S - 1) / S : 1;
+  const int64_t tile_rows = per_seq < 32 || p.key_rows != 32 ? (per_seq < 32 ? per_seq : 32)
+                                                             : (per_seq < kRowTile ? per_seq : kRowTile);
+  p.min_chunk = (int)((8 * tile_rows + kMinChunk - 1) / kMinChunk * kMinChunk);
+  const int64_t items = (packed && p.key_rows == 32 ? r.row_tiles + (per_seq <= 32 ? S : 0) : r.key_tiles) * heads;
+  const int64_t cap = ((int64_t)p.s.max_pages * p.s.page_size + p.min_chunk - 1) / p.min_chunk;
+  int64_t want = kSlots * (per_seq < kRowTile ? 4 : 1) / (items > 0 ? items : 1);
   if (want > cap) want = cap;
-  if (want > 256) want = 256;
-  return want < 1 ? 1 : (int)want;
+  if (want > kMaxSplits) want = kMaxSplits;
+  p.splits = want < 1 ? 1 : (int)want;
+  return r;
 }
 
 template <typename T, int D>
-int launch_attention(const AttnParams& p, hipStream_t s) {
-  const bool packed = p.s.cu != nullptr;
+int launch_attention(AttnParams p, hipStream_t s) {
+  const Plan r = plan(p);
   const int64_t per_tile = (int64_t)p.kv_heads * p.splits;
-  const int64_t keys = tile_bound(p.s.num_tokens, p.s.num_seqs, p.group.d, 32, packed) * per_tile;
-  const int64_t rows = packed ? tile_bound(p.s.num_tokens, p.s.num_seqs, p.group.d, kRowTile, true) * per_tile : 0;
-  const int64_t join = (int64_t)p.s.num_tokens * p.q_heads;
-  PKDA_REQUIRE(keys <= INT32_MAX && rows <= INT32_MAX && join <= INT32_MAX, PKDA_EINVAL, "%d tokens of %d heads",
-               p.s.num_tokens, p.q_heads);
-  if (rows) {
-    if (p.s.page_size % (64 / Geo<T, D>::NC) == 0)
-      hipLaunchKernelGGL((paged_attention_rows_kernel<T, D, true>), dim3((unsigned)rows), dim3(kThreads), 0, s, p);
-    else
-      hipLaunchKernelGGL((paged_attention_rows_kernel<T, D, false>), dim3((unsigned)rows), dim3(kThreads), 0, s, p);
-    if (int st = launch_status("pkda_paged_attention(rows)")) return st;
-  }
-  hipLaunchKernelGGL((paged_attention_keys_kernel<T, D>), dim3((unsigned)keys), dim3(kThreads), 0, s, p);
-  if (int st = launch_status("pkda_paged_attention(keys)")) return st;
-  if (p.splits > 1) {
-    hipLaunchKernelGGL((paged_attention_join_kernel<T, D>), dim3((unsigned)join), dim3(kThreads), 0, s, p);
-    return launch_status("pkda_paged_attention(join)");
-  }
-  return 0;
+  const int64_t blocks = (r.row_tiles + r.key_tiles) * per_tile;
+  const int64_t rows = (int64_t)p.s.num_tokens * p.q_heads;
+  PKDA_REQUIRE(blocks <= INT32_MAX && rows <= INT32_MAX, PKDA_EINVAL, "%d tokens of %d heads", p.s.num_tokens,
+               p.q_heads);
+  p.row_blocks = (unsigned)(r.row_tiles * per_tile);
+  const dim3 grid((unsigned)blocks), block(kThreads);
+  if (!p.s.cu)
+    hipLaunchKernelGGL((paged_attention_token_kernel<T, D>), grid, block, 0, s, p);
+  else if (p.s.page_size % (64 / Geo<T, D>::NC) == 0)
+    hipLaunchKernelGGL((paged_attention_kernel<T, D, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((paged_attention_kernel<T, D, false>), grid, block, 0, s, p);
+  if (int st = launch_status("pkda_paged_attention")) return st;
+  if (p.splits == 1) return 0;
+  if (rows < 2 * kSlots)
+    hipLaunchKernelGGL((paged_attention_join_kernel<T, D, kWaves>), dim3((unsigned)rows), block, 0, s, p);
+  else
+    hipLaunchKernelGGL((paged_attention_join_kernel<T, D, 1>), dim3((unsigned)((rows + kWaves - 1) / kWaves)), block, 0, s, p);
+  return launch_status("pkda_paged_attention(join)");
 }
 
 template <typename T>
@@ -794,7 +859,7 @@ int attention_sizes(const pkda_paged_attention_args* a, AttnParams& p) {
   p.group = FastDiv::make((uint32_t)(a->q_heads / a->kv_heads));
   PKDA_REQUIRE((int64_t)a->num_tokens * p.group.d <= INT32_MAX, PKDA_EINVAL, "%d tokens of %d heads", a->num_tokens,
                a->q_heads);
-  p.splits = plan_splits(p);
+  plan(p);
   return 0;
 }
 

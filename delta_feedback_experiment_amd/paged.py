@@ -52,55 +52,54 @@ class PagedKV:
 def _check_cache(name: str, x: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seq_lens: Tensor,
                  cu_seqlens: Tensor | None) -> None:
     """The checks the two operators share; ``x`` is a token tensor."""
-    if x.dim() != 3:
-        raise ValueError(f"{name} [tokens, heads, head_dim] expected, got {tuple(x.shape)}")
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
-        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must be one "
+    shape, pages, dtype, lens = x.shape, k_pages.shape, x.dtype, seq_lens.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name} [tokens, heads, head_dim] expected, got {tuple(shape)}")
+    if len(pages) != 4 or pages != v_pages.shape:
+        raise ValueError(f"k_pages {tuple(pages)} and v_pages {tuple(v_pages.shape)} must be one "
                          "[pages, page_size, kv_heads, head_dim] shape")
-    if x.dtype != k_pages.dtype or x.dtype != v_pages.dtype:
-        raise ValueError(f"{name} {x.dtype} and the pages {k_pages.dtype}, {v_pages.dtype} must share one dtype")
-    if x.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"float32 or bfloat16 expected, not {x.dtype}")
-    D = k_pages.shape[3]
-    if x.shape[2] != D or D not in HEAD_DIMS:
-        raise ValueError(f"head_dim {x.shape[2]} of {name} and {D} of the pages: one of {HEAD_DIMS} expected")
-    if k_pages.shape[1] < 1 or k_pages.shape[2] < 1:
-        raise ValueError(f"pages {tuple(k_pages.shape)} hold nothing")
-    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1:
+    if dtype != k_pages.dtype or dtype != v_pages.dtype:
+        raise ValueError(f"{name} {dtype} and the pages {k_pages.dtype}, {v_pages.dtype} must share one dtype")
+    if dtype != torch.bfloat16 and dtype != torch.float32:
+        raise ValueError(f"float32 or bfloat16 expected, not {dtype}")
+    _, R, H, D = pages
+    if shape[2] != D or D not in HEAD_DIMS:
+        raise ValueError(f"head_dim {shape[2]} of {name} and {D} of the pages: one of {HEAD_DIMS} expected")
+    if R < 1 or H < 1:
+        raise ValueError(f"pages {tuple(pages)} hold nothing")
+    if seq_lens.dtype != torch.int32 or len(lens) != 1:
         raise ValueError("seq_lens must be int32 [sequences]")
-    S = seq_lens.shape[0]
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != S:
+    S, table = lens[0], page_table.shape
+    if page_table.dtype != torch.int32 or len(table) != 2 or table[0] != S:
         raise ValueError(f"page_table must be int32 [{S}, pages of a sequence]")
     if cu_seqlens is None:
-        if x.shape[0] != S:
-            raise ValueError(f"{x.shape[0]} tokens of {S} sequences need cu_seqlens")
+        if shape[0] != S:
+            raise ValueError(f"{shape[0]} tokens of {S} sequences need cu_seqlens")
     elif cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (S + 1,):
         raise ValueError(f"cu_seqlens must be int32 [{S + 1}]")
-    for pages in (k_pages, v_pages):
-        if not _dense_pages(pages):
+    for t in (k_pages, v_pages):
+        stride = t.stride()
+        if (stride[3] != 1 or stride[2] != D or stride[1] != H * D or not _aligned(t, stride[0])) and t.numel():
             raise ValueError("every page must be dense, in whole 16 bytes")
 
 
-def _dense_pages(pages: Tensor) -> bool:
-    _, R, H, D = pages.shape
-    return (pages.stride()[1:] == (H * D, D, 1) and _aligned(pages, pages.stride(0))) or pages.numel() == 0
-
-
 def _aligned(t: Tensor, stride: int) -> bool:
-    # the storage of fake tensors has no address: the offset is what a view adds to it
-    return stride * t.element_size() % 16 == 0 and t.storage_offset() * t.element_size() % 16 == 0
+    # fake tensors have no address: the offset is what a view adds to its storage
+    return (stride | t.storage_offset()) * t.element_size() % 16 == 0
 
 
 def _rows(t: Tensor) -> Tensor:
     """Tokens as the kernels read them: heads dense, tokens any whole 16 bytes apart."""
-    H, D = t.shape[1:]
-    if t.stride(2) == 1 and (t.stride(1) == D or H == 1) and _aligned(t, t.stride(0)) and t.stride(0) >= 0:
+    _, H, D = t.shape
+    token, head, channel = t.stride()
+    if channel == 1 and (head == D or H == 1) and token >= 0 and _aligned(t, token):
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _ints(t: Tensor) -> Tensor:
-    return t if t.stride(-1) == 1 and t.stride(0) >= 0 else t.contiguous()
+    stride = t.stride()
+    return t if stride[-1] == 1 and stride[0] >= 0 else t.contiguous()
 
 
 def validate_pages(page_table: Tensor, seq_lens: Tensor, cu_seqlens: Tensor | None, num_tokens: int, num_pages: int,
