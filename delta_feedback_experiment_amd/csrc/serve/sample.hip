@@ -299,6 +299,7 @@ __device__ __forceinline__ void sort_list(Lds& lds, int n) {
   const uint64_t mine = lds.list[i];
   const int quarter = (n + 3) / 4;
   int rank = 0;
+#pragma unroll 8
   for (int j = part * quarter; j < min(n, (part + 1) * quarter); ++j) rank += lds.list[j] > mine;
   lds.ranks[part][i] = rank;
   __syncthreads();
@@ -343,6 +344,25 @@ __device__ __forceinline__ int take_places(int* count) {
   if (before == 0) at = atomicAdd(count, __popcll(active));
   return __builtin_amdgcn_readfirstlane(at) + before;
 }
+// The same within each wave, k / 16 of its threads, and the least of the waves'
+// numbers: no counts to exchange, for a few more logits that reach it.
+__device__ __forceinline__ uint32_t reached_by_waves(uint32_t mine, int k, Lds& lds) {
+  const int need = (k + kWaves - 1) / kWaves;
+  uint32_t found = 0;
+#pragma unroll
+  for (int bit = 15; bit >= 0; --bit) {
+    const uint32_t t = found | 1u << bit;
+    if (__popcll(__ballot(mine >= t)) >= need) found = t;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds.wave_f[threadIdx.x >> 6] = (float)found;
+  __syncthreads();
+  float least = lds.wave_f[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) least = fminf(least, lds.wave_f[i]);
+  return (uint32_t)least;
+}
+
 // The indices of the logits that reach least, into the candidates; returns how
 // many there are (more than kCandidates: the list is not complete).  Four
 // vectors' comparisons make a lane's mask, one addition a wave the places of all.
@@ -359,6 +379,19 @@ __device__ __forceinline__ int gather(const RowData<T>& row, float least, Lds& l
 #pragma unroll
       for (int j = 0; j < L::N; ++j) mask |= L::get(x[u], j) >= least ? 1u << (u * L::N + j) : 0u;
     const int n = __popc(mask);
+    const uint64_t any = __ballot(n != 0);
+    if (any == 0) return;
+    int at = 0;
+    if (__popcll(any) <= 8) {
+      if (n != 0) at = atomicAdd(&lds.count, n);
+      while (mask) {
+        const int b = __builtin_ctz(mask);
+        mask &= mask - 1;
+        if (at < kCandidates) lds.candidates[at] = (c + b / L::N * kThreads) * L::N + b % L::N;
+        ++at;
+      }
+      return;
+    }
     // the lanes before this one have sum over bits b of 2^b times those whose n has it
     int before = 0, all = 0;
 #pragma unroll
@@ -367,8 +400,6 @@ __device__ __forceinline__ int gather(const RowData<T>& row, float least, Lds& l
       before += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0)) << b;
       all += __popcll(has) << b;
     }
-    if (all == 0) return;
-    int at = 0;
     if (before == 0) {  // the first lanes: one of them, of the active ones, adds
       const uint64_t first = __ballot(true);
       if ((int)(threadIdx.x & 63) == __builtin_ctzll(first)) at = atomicAdd(&lds.count, all);
@@ -401,7 +432,7 @@ template <typename T> struct Source {
       row.each(f);
       return;
     }
-    constexpr int U = 4;
+    constexpr int U = 8;
     for (int i = threadIdx.x; i < n; i += U * kThreads) {
       int at[U];
       float x[U];
@@ -762,25 +793,36 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     const float t = z + g;
     if (t > -INFINITY) pick = max_key(pick, ((uint64_t)float_key(fminf(t, kMaxFloat)) << 32) | (uint32_t)~i);
   };
-  const auto score = [&](uint64_t key) {
+  const auto score = [&](uint64_t key, float g) {
     const float z = s.z(key_logit(key));
-    const int i = key_index(key);
-    if (min_p <= 0.f || expf(z) >= min_p) take(z, row.noise[i], i);
+    if (min_p <= 0.f || expf(z) >= min_p) take(z, g, key_index(key));
   };
-
   // the candidates that a prefix ending with low keeps
   const auto score_candidates = [&](int n, uint64_t low) {
-    const Source<T> from = {row, lds.candidates, n};
-    from.each([&](float x, int i) {
-      const uint64_t key = order_key(x, i);
-      if (key >= low) score(key);
-    });
+    constexpr int U = 4;
+    for (int i = threadIdx.x; i < n; i += U * kThreads) {
+      int at[U];
+      float x[U], g[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) at[u] = (int)lds.candidates[i + u * kThreads < n ? i + u * kThreads : i];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u] = row.one(at[u]);
+        g[u] = row.noise[at[u]];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // (one twice: no harm)
+        const uint64_t key = order_key(x[u], at[u]);
+        if (key >= low) score(key, g[u]);
+      }
+    }
   };
 
   if (temperature > 0.f) {
     bool done = false;
     if (k > 0 && k <= kList) {
-      const float least = key_float(max(reached_by(float_key(mine) >> 16, k, lds) << 16, kMinKey));
+      const float least = key_float(max((k <= kRanked ? reached_by_waves(float_key(mine) >> 16, k, lds)
+                                                       : reached_by(float_key(mine) >> 16, k, lds)) << 16, kMinKey));
       const int n = gather(row, least, lds);
       if (n <= kList) {
         if ((int)threadIdx.x < n) {
@@ -795,7 +837,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
           const double before = block_scan(keep ? (double)s.weight(key_logit(key)) : 0., lds.wave_d, held);
           keep = keep && (before < (double)top_p * held || threadIdx.x == 0);
         }
-        if (keep) score(key);
+        if (keep) score(key, row.noise[key_index(key)]);
         done = true;
       }
     }
