@@ -208,7 +208,13 @@ __device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& 
   tile.first = base + (int)p.group.div((uint32_t)row0);
   tile.last = base + (int)p.group.div((uint32_t)min(rows - 1, row0 + M - 1));
   tile.keys = p.s.num_pages == 0 ? 0 : max(0, tile.last + 1);
-  tile.chunk = split_chunk(p, tile.span.len);
+  // the same in every lane, and in scalar registers once it is said
+  const auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  tile.span = {same(tile.span.first), same(tile.span.count), same(tile.span.len)};
+  tile.first = same(tile.first);
+  tile.last = same(tile.last);
+  tile.keys = same(tile.keys);
+  tile.chunk = same(split_chunk(p, tile.span.len));
   tile.direct = tile.span.len <= tile.chunk;
   return true;
 }
@@ -510,8 +516,8 @@ constexpr int kRowTile = 32 * kWaves;
 constexpr int kKeyTile = 64;
 
 // WHOLE: the rows that a wave stages at a time, 64 / NC keys, lie in one page
-// (the page size is a multiple of them): their page is looked up once a wave,
-// in scalar registers, and a lane's address is that plus a constant.
+// (the page size is a multiple of them): a load's address is the page's, in
+// scalar registers, and a lane's constant part.
 template <typename T, int D> struct RowsLds {
   __align__(16) char kv[4 * kKeyTile * Geo<T, D>::RB];  // two stages of K, V
   // of tile t % 3: its keys with values that are not finite, and those without a page
@@ -553,39 +559,57 @@ __device__ __forceinline__ void attend_rows(const AttnParams& p, unsigned block,
 
   const int tiles = k1 > k0 ? (k1 - k0 + kKeyTile - 1) / kKeyTile : 0;
   const int srow = tid / G::NC, schunk = tid % G::NC;
-  const T* kb = static_cast<const T*>(p.k_pages) + (int64_t)kvh * D + schunk * G::EC;
-  const T* vb = static_cast<const T*>(p.v_pages) + (int64_t)kvh * D + schunk * G::EC;
   const int row_stride = p.kv_heads * D;
+  // a lane's own part of an address: its chunk of its row of the wave's rows
+  const uint32_t lane_off = (uint32_t)(WHOLE ? (srow - RW * w) * row_stride : 0) * sizeof(T) + schunk * 16;
+  const char* kb = static_cast<const char*>(p.k_pages) + (int64_t)kvh * G::RB;
+  const char* vb = static_cast<const char*>(p.v_pages) + (int64_t)kvh * G::RB;
+  const int64_t k_page = p.k_page_stride * (int64_t)sizeof(T), v_page = p.v_page_stride * (int64_t)sizeof(T);
 
-  int page[NI], prow[NI];
+  // The table's entries of the next tile, looked up a tile ahead: of this thread's
+  // rows, or (WHOLE) of the wave's, one a lane, so that all are found at once.
+  constexpr int NL = WHOLE ? 1 : NI;
+  int page[NL], prow[NL];
   const auto look = [&](int t) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      if constexpr (WHOLE) {
-        const int key = min(k0 + kKeyTile * t + RI * i + RW * w, (k1 - 1) / RW * RW);
-        page[i] = page_entry(p.s, tile.n, key, &prow[i]);
-      } else {
-        const int key = k0 + kKeyTile * t + RI * i + srow;
-        page[i] = page_entry(p.s, tile.n, min(key, k1 - 1), &prow[i]);
-      }
+    for (int i = 0; i < NL; ++i) {
+      const int key = k0 + kKeyTile * t + (WHOLE ? RI * (lane & (NI - 1)) + RW * w : RI * i + srow);
+      page[i] = page_entry(p.s, tile.n, min(key, WHOLE ? (k1 - 1) / RW * RW : k1 - 1), &prow[i]);
     }
   };
-  const int lane_off = WHOLE ? (srow - RW * w) * row_stride : 0;
   u32x4 k[NI], v[NI];
   uint32_t gone = 0;  // this thread's staged rows that are not there, one bit each
   const auto load = [&](int t) {
-    const T *ks[NI], *vs[NI];
+    const char *ks[NI], *vs[NI];
     gone = 0;
+    uint64_t ko[NL], vo[NL];
+    bool here[NL];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      int at = page[i], r = prow[i];
-      if constexpr (WHOLE) at = __builtin_amdgcn_readfirstlane(at);
-      if (!page_exists(p.s, at)) {
-        gone |= 1u << i;
-        at = r = 0;
+    for (int i = 0; i < NL; ++i) {
+      here[i] = page_exists(p.s, page[i]);
+      const uint32_t at = here[i] ? page[i] : 0, r = here[i] ? prow[i] : 0;
+      const uint64_t off = (uint64_t)r * (uint32_t)(row_stride * (int)sizeof(T));
+      ko[i] = at * (uint64_t)k_page + off;
+      vo[i] = at * (uint64_t)v_page + off;
+    }
+    if constexpr (WHOLE) {
+      const auto of_lane = [](uint64_t x, int i) {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, i) |
+               (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), i) << 32;
+      };
+      gone = ~(uint32_t)__ballot(here[0]) & ((1u << NI) - 1);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        ks[i] = kb + of_lane(ko[0], i);
+        vs[i] = vb + of_lane(vo[0], i);
       }
-      ks[i] = kb + at * p.k_page_stride + (int64_t)r * row_stride;
-      vs[i] = vb + at * p.v_page_stride + (int64_t)r * row_stride;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        gone |= (here[i] ? 0u : 1u) << i;
+        ks[i] = kb + ko[i];
+        vs[i] = vb + vo[i];
+      }
     }
     if (t + 1 < tiles) look(t + 1);  // before the keys' loads, which it would otherwise wait for
 #pragma unroll
