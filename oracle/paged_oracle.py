@@ -72,3 +72,31 @@ def attention_reference(q, k_pages, v_pages, page_table, seq_lens, cu_seqlens=No
             lse[t, h] = torch.logsumexp(s, 0)
             o[t, h] = torch.softmax(s, 0) @ v[:, h // (Hq // Hkv)]
     return o, lse
+
+
+def attention_of_sequences(q, k_pages, v_pages, page_table, seq_lens, cu_seqlens, scale=None):
+    """``attention_reference`` a sequence at a time, for longer ones."""
+    N, Hq, D = q.shape
+    P, R, Hkv = k_pages.shape[:3]
+    scale = D ** -0.5 if scale is None else scale
+    o, lse = torch.zeros(N, Hq, D, dtype=torch.float64), torch.full((N, Hq), -torch.inf, dtype=torch.float64)
+    for n, length in enumerate(seq_lens.tolist()):
+        first, new = int(cu_seqlens[n]), int(cu_seqlens[n + 1] - cu_seqlens[n])
+        if new == 0 or length <= 0:
+            continue
+        at = torch.arange(length)
+        page = page_table[n, at // R].long()
+        there = (page >= 0) & (page < P)
+        page, row = page.clamp(0, P - 1), at % R
+        sees = (at <= (length - new + torch.arange(new))[:, None]) & there  # [new, length]
+        for h in range(Hkv):
+            k, v = k_pages[page, row, h].double(), v_pages[page, row, h].double()
+            k, v = (torch.where(there[:, None], x, 0.0) for x in (k, v))
+            heads = slice(h * (Hq // Hkv), (h + 1) * (Hq // Hkv))
+            s = scale * (q[first:first + new, heads].double() @ k.T)  # [new, group, length]
+            s = s.masked_fill(~sees[:, None], -torch.inf)
+            top = torch.logsumexp(s, -1)
+            lse[first:first + new, heads] = top
+            pr = torch.exp(s - top.clamp(min=torch.finfo(torch.float64).min)[..., None])
+            o[first:first + new, heads] = pr @ v
+    return o, lse

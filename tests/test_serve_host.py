@@ -210,6 +210,20 @@ def test_paged_oracle_is_causal_attention():
     assert torch.allclose(lse, s.logsumexp(-1).t(), atol=1e-12)
 
 
+def test_paged_oracle_by_sequence_equals_by_token():
+    gen = torch.Generator().manual_seed(3)
+    lens, new = [7, 0, 12, 5], [3, 0, 12, 9]
+    cu = torch.tensor([0, 3, 3, 15, 24], dtype=torch.int32)
+    table = torch.randperm(16, generator=gen).int().view(4, 4)
+    table[2, 1], table[0, 0] = -1, 99
+    q = torch.randn(26, 4, 8, generator=gen)
+    k, v = (torch.randn(16, 4, 2, 8, generator=gen) for _ in range(2))
+    args = (q, k, v, table, torch.tensor(lens, dtype=torch.int32), cu, 0.7)
+    for a, b in zip(paged_oracle.attention_reference(*args), paged_oracle.attention_of_sequences(*args)):
+        torch.testing.assert_close(a, b, rtol=1e-12, atol=1e-12)
+
+
+
 def test_sample_oracle_settings():
     l = torch.tensor([1.0, 3.0, 2.0, 3.0, 0.0])
     assert sample_oracle.kept_tokens(l, 1.0)[0].tolist() == [1, 3, 2, 0, 4]
