@@ -181,24 +181,10 @@ __device__ __forceinline__ int split_chunk(const AttnParams& p, int len) {
 __host__ __device__ inline int64_t tile_bound(int64_t tokens, int64_t seqs, int64_t group, int M, bool packed) {
   return packed ? tokens * group / M + seqs + 1 : seqs * ((group + M - 1) / M);
 }
+// Tile `local` of M rows of sequence tile.n.
 template <int M>
-__device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& tile) {
+__device__ __forceinline__ bool fill_tile(const AttnParams& p, int local, Tile& tile) {
   const int group = (int)p.group.d;
-  int local;
-  if (M == 32 && p.s.cu && p.key_rows == 32) {  // one tile a sequence
-    tile.n = (int)t;
-    local = 0;
-  } else if (p.s.cu) {
-    const auto begin = [&](int n) -> int64_t {
-      return (n == 0 ? 0 : (int64_t)clamp_int(p.s.cu[n], 0, p.s.num_tokens) * group / M) + n;
-    };
-    tile.n = wave_upper(p.s.num_seqs, t, begin);
-    local = (int)(t - begin(tile.n));
-  } else {
-    const int per = (group + M - 1) / M;
-    tile.n = (int)(t / per);
-    local = (int)(t - (int64_t)tile.n * per);
-  }
   tile.span = seq_span(p.s, tile.n);
   const int64_t rows = (int64_t)tile.span.count * group, row0 = (int64_t)local * M;
   if (row0 >= rows) return false;
@@ -217,6 +203,72 @@ __device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& 
   tile.chunk = same(split_chunk(p, tile.span.len));
   tile.direct = tile.span.len <= tile.chunk;
   return true;
+}
+template <int M>
+__device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& tile) {
+  const int group = (int)p.group.d;
+  int local;
+  if (M == 32 && p.s.cu && p.key_rows == 32) {  // one tile a sequence
+    tile.n = (int)t;
+    local = 0;
+  } else if (p.s.cu) {
+    const auto begin = [&](int n) -> int64_t {
+      return (n == 0 ? 0 : (int64_t)clamp_int(p.s.cu[n], 0, p.s.num_tokens) * group / M) + n;
+    };
+    tile.n = wave_upper(p.s.num_seqs, t, begin);
+    local = (int)(t - begin(tile.n));
+  } else {
+    const int per = (group + M - 1) / M;
+    tile.n = (int)(t / per);
+    local = (int)(t - (int64_t)tile.n * per);
+  }
+  return fill_tile<M>(p, local, tile);
+}
+
+// The wave's sum of x, in every lane.
+__device__ __forceinline__ int wave_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false);   // quad [1,0,3,2]
+  x += __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false);   // quad [2,3,0,1]
+  x += __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false);  // half-row mirror
+  x += __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false);  // row mirror
+  auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = r[0] + r[1];
+  r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __builtin_amdgcn_readfirstlane(r[0] + r[1]);
+}
+
+// The t-th of the M-row tiles of sequences of more than key_rows rows, those
+// with the most keys first: lane n has sequence n (fewer than 64).  A tile's
+// level is its last row counted from the sequence's first position, in tiles;
+// a sequence has one tile a level from lo up, so the tiles from a level up are
+// counted by one sum over the wave, and the level of the t-th by bisection.
+template <int M>
+__device__ __forceinline__ bool find_longest(const AttnParams& p, int t, Tile& tile) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, tiles = 0;
+  if (lane <= p.s.num_seqs) {
+    const SeqSpan span = seq_span(p.s, lane);
+    const int64_t rows = (int64_t)span.count * p.group.d;
+    if (rows > p.key_rows) tiles = (int)((rows + M - 1) / M);
+    lo = (int)min((int64_t)max(0, span.len - span.count) * p.group.d / M, (int64_t)1 << 30);
+  }
+  if (t >= wave_sum(tiles)) return false;
+  const auto from = [&](int level) { return wave_sum(clamp_int(lo + tiles - level, 0, tiles)); };
+  int x = 0, y = lo + tiles;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) y = max(y, __shfl_xor(y, o));
+  y = __builtin_amdgcn_readfirstlane(y);
+  while (y - x > 1) {  // from(x) > t >= from(y)
+    const int mid = x + (y - x) / 2;
+    if (from(mid) > t) x = mid;
+    else y = mid;
+  }
+  // of the level's tiles the (t - from(y))-th; the sum by all lanes, outside the condition
+  const int place = t - from(y);
+  const bool mine = (lo <= x) & (x < lo + tiles);
+  const uint64_t at = __ballot(mine);
+  tile.n = __builtin_ctzll(__ballot(mine & (__popcll(at & ((1ull << lane) - 1)) == place)));
+  return fill_tile<M>(p, x - __builtin_amdgcn_readlane(lo, tile.n), tile);
 }
 
 // One query row of a lane.
@@ -539,8 +591,9 @@ __device__ __forceinline__ void attend_rows(const AttnParams& p, unsigned block,
   const int split = rest % p.splits;
   const int64_t bound = tile_bound(p.s.num_tokens, p.s.num_seqs, p.group.d, kRowTile, true);
   Tile tile;
-  if (!find_tile<kRowTile>(p, bound - 1 - rest / p.splits, tile)) return;  // the longest first
-  if (tile.rows <= p.key_rows) return;                                     // the other form's
+  const int t = rest / p.splits;
+  if (p.s.num_seqs < 64 ? !find_longest<kRowTile>(p, t, tile) : !find_tile<kRowTile>(p, bound - 1 - t, tile)) return;
+  if (tile.rows <= p.key_rows) return;  // the other form's
   const int k0 = split * tile.chunk, k1 = min(k0 + tile.chunk, tile.keys);
   if (split > 0 && (k0 >= tile.keys || tile.direct)) return;
 
