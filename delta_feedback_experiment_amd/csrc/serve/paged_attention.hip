@@ -181,11 +181,11 @@ __device__ __forceinline__ int split_chunk(const AttnParams& p, int len) {
 __host__ __device__ inline int64_t tile_bound(int64_t tokens, int64_t seqs, int64_t group, int M, bool packed) {
   return packed ? tokens * group / M + seqs + 1 : seqs * ((group + M - 1) / M);
 }
-// Tile `local` of M rows of sequence tile.n.
+// Tile `local` of M rows of sequence tile.n, whose span is given.
 template <int M>
-__device__ __forceinline__ bool fill_tile(const AttnParams& p, int local, Tile& tile) {
+__device__ __forceinline__ bool fill_tile(const AttnParams& p, int local, const SeqSpan& span, Tile& tile) {
   const int group = (int)p.group.d;
-  tile.span = seq_span(p.s, tile.n);
+  tile.span = span;
   const int64_t rows = (int64_t)tile.span.count * group, row0 = (int64_t)local * M;
   if (row0 >= rows) return false;
   tile.rows = (int)rows;
@@ -222,7 +222,7 @@ __device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& 
     tile.n = (int)(t / per);
     local = (int)(t - (int64_t)tile.n * per);
   }
-  return fill_tile<M>(p, local, tile);
+  return fill_tile<M>(p, local, seq_span(p.s, tile.n), tile);
 }
 
 // The wave's sum of x, in every lane.
@@ -246,8 +246,9 @@ template <int M>
 __device__ __forceinline__ bool find_longest(const AttnParams& p, int t, Tile& tile) {
   const int lane = threadIdx.x & 63;
   int lo = 0, tiles = 0;
+  SeqSpan span = {0, 0, 0};
   if (lane <= p.s.num_seqs) {
-    const SeqSpan span = seq_span(p.s, lane);
+    span = seq_span(p.s, lane);
     const int64_t rows = (int64_t)span.count * p.group.d;
     if (rows > p.key_rows) tiles = (int)((rows + M - 1) / M);
     lo = (int)min((int64_t)max(0, span.len - span.count) * p.group.d / M, (int64_t)1 << 30);
@@ -268,7 +269,8 @@ __device__ __forceinline__ bool find_longest(const AttnParams& p, int t, Tile& t
   const bool mine = (lo <= x) & (x < lo + tiles);
   const uint64_t at = __ballot(mine);
   tile.n = __builtin_ctzll(__ballot(mine & (__popcll(at & ((1ull << lane) - 1)) == place)));
-  return fill_tile<M>(p, x - __builtin_amdgcn_readlane(lo, tile.n), tile);
+  const auto its = [&](int v) { return __builtin_amdgcn_readlane(v, tile.n); };
+  return fill_tile<M>(p, x - its(lo), {its(span.first), its(span.count), its(span.len)}, tile);
 }
 
 // One query row of a lane.
@@ -301,11 +303,14 @@ __device__ __forceinline__ Row load_row(const AttnParams& p, const Tile& tile, i
       for (int i = 0; i < G::NP; ++i) q[i] ^= sign;
     }
   }
-  // the queries arrive before the loop over the keys: waits inside it would hold
-  // the keys that are on their way
-#pragma unroll
-  for (int i = 0; i < G::NP; ++i) asm volatile("" : "+v"(q[i]));
   return row;
+}
+// The queries arrive before the loop over the keys, and after the first keys are
+// asked for: waits inside the loop would hold the keys that are on their way.
+template <int N>
+__device__ __forceinline__ void arrived(u32x4 (&q)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(q[i]));
 }
 
 // A row's softmax while its keys pass.
@@ -426,11 +431,6 @@ __device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block,
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 31, half = lane >> 5;
-  u32x4 q[G::NP];
-  const Row row = load_row<T, D>(p, tile, kvh, tile.row0 + col, half, q);
-  Running<G::DT> run;
-  run.init();
-
   char* sv = s_buf + w * 32 * G::RB;
   const int tiles = k1 > k0 ? (k1 - k0 + 31) / 32 : 0;
   const T* kb = static_cast<const T*>(p.k_pages) + (int64_t)kvh * D + half * G::EC;
@@ -455,14 +455,19 @@ __device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block,
   };
 
   int page = 0, r = 0;
+  if (w < tiles) page = look(w, r);
+  u32x4 q[G::NP];
+  const Row row = load_row<T, D>(p, tile, kvh, tile.row0 + col, half, q);
+  Running<G::DT> run;
+  run.init();
   if (w < tiles) {
-    page = look(w, r);
     int page1 = 0, r1 = 0;
     if (w + kWaves < tiles) page1 = look(w + kWaves, r1);
     load(w, page, r);
     page = page1;
     r = r1;
   }
+  arrived(q);
   for (int t = w; t < tiles; t += kWaves) {
     const int key0 = k0 + 32 * t;
     const uint32_t there = (uint32_t)__ballot(here);
@@ -599,17 +604,12 @@ __device__ __forceinline__ void attend_rows(const AttnParams& p, unsigned block,
 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int col = lane & 31, half = lane >> 5;
-  u32x4 q[G::NP];
   const int wrow0 = tile.row0 + 32 * w;
-  const Row row = load_row<T, D>(p, tile, kvh, wrow0 + col, half, q);
   // positions of the wave's first and last live row
   const int base = tile.span.len - tile.span.count;
   const bool wlive = wrow0 < tile.rows;
   const int wfirst = wlive ? base + (int)p.group.div((uint32_t)wrow0) : -1;
   const int wlast = wlive ? base + (int)p.group.div((uint32_t)min(tile.rows - 1, wrow0 + 31)) : -1;
-  Running<G::DT> run;
-  run.init();
-
   const int tiles = k1 > k0 ? (k1 - k0 + kKeyTile - 1) / kKeyTile : 0;
   const int srow = tid / G::NC, schunk = tid % G::NC;
   const int row_stride = p.kv_heads * D;
@@ -700,13 +700,16 @@ __device__ __forceinline__ void attend_rows(const AttnParams& p, unsigned block,
       *reinterpret_cast<u32x4*>(sk + kTileBytes + at) = v[i];
     }
   };
+  if (tiles > 0) look(0);
+  u32x4 q[G::NP];
+  const Row row = load_row<T, D>(p, tile, kvh, wrow0 + col, half, q);
+  Running<G::DT> run;
+  run.init();
   if (tid < 12) s_odd[tid >> 2][tid & 3] = 0;
+  if (tiles > 0) load(0);
+  arrived(q);
   __syncthreads();
-  if (tiles > 0) {
-    look(0);
-    load(0);
-    stage(0, 0);
-  }
+  if (tiles > 0) stage(0, 0);
   __syncthreads();
   int slot = 0;
   for (int t = 0; t < tiles; ++t) {
