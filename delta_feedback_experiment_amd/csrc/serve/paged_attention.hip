@@ -42,6 +42,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 struct AttnParams {
@@ -225,16 +226,20 @@ __device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& 
   return fill_tile<M>(p, local, seq_span(p.s, tile.n), tile);
 }
 
-// The wave's sum of x, in every lane.
-__device__ __forceinline__ int wave_sum(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false);   // quad [1,0,3,2]
-  x += __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false);   // quad [2,3,0,1]
-  x += __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false);  // half-row mirror
-  x += __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false);  // row mirror
+// f over the wave's x.
+template <typename F>
+__device__ __forceinline__ int wave_join(int x, F f) {
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false));   // quad [1,0,3,2]
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false));   // quad [2,3,0,1]
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false));  // half-row mirror
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false));  // row mirror
   auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  x = r[0] + r[1];
+  x = f((int)r[0], (int)r[1]);
   r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  return __builtin_amdgcn_readfirstlane(r[0] + r[1]);
+  return __builtin_amdgcn_readfirstlane(f((int)r[0], (int)r[1]));
+}
+__device__ __forceinline__ int wave_sum(int x) {
+  return wave_join(x, [](int a, int b) { return a + b; });
 }
 
 // The t-th of the M-row tiles of sequences of more than key_rows rows, those
@@ -255,10 +260,7 @@ __device__ __forceinline__ bool find_longest(const AttnParams& p, int t, Tile& t
   }
   if (t >= wave_sum(tiles)) return false;
   const auto from = [&](int level) { return wave_sum(clamp_int(lo + tiles - level, 0, tiles)); };
-  int x = 0, y = lo + tiles;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) y = max(y, __shfl_xor(y, o));
-  y = __builtin_amdgcn_readfirstlane(y);
+  int x = 0, y = wave_join(lo + tiles, [](int a, int b) { return max(a, b); });
   while (y - x > 1) {  // from(x) > t >= from(y)
     const int mid = x + (y - x) / 2;
     if (from(mid) > t) x = mid;
@@ -358,6 +360,36 @@ template <int DT> struct Running {
 };
 
 __device__ __forceinline__ int key_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+// A row of the output.  A lane holds four channels of every eight; in BF16 the
+// halves exchange theirs, eight channels for eight, and store 16 bytes.
+template <typename T, int D>
+__device__ __forceinline__ void store_row(T* dst, const f32x16 (&o)[D / 32], float f, int half) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int r = 0; r < 16; r += 8) {
+        u32x4 x;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const auto pair = [&](int at) -> uint32_t {
+            return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(o[dt][at] * f), static_cast<__bf16>(o[dt][at + 1] * f)});
+          };
+          const auto y = __builtin_amdgcn_permlane32_swap(pair(r + 2 * i), pair(r + 4 + 2 * i), false, false);
+          x[i] = y[0];
+          x[2 + i] = y[1];
+        }
+        *reinterpret_cast<u32x4*>(dst + 32 * dt + 2 * r + 8 * half) = x;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<f32x4_t*>(dst + 32 * dt + key_of(r, half)) =
+            f32x4_t{o[dt][r] * f, o[dt][r + 1] * f, o[dt][r + 2] * f, o[dt][r + 3] * f};
+    }
+  }
+}
 
 // What values that are not finite add to the rows that see them (the products
 // ran with zeros there, so that a row that does not see them stays what it is):
@@ -761,13 +793,7 @@ __device__ __forceinline__ void attend_rows(const AttnParams& p, unsigned block,
   const float l = join_halves(run.l, [](float a, float b) { return a + b; });
   if (tile.direct) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* dst = static_cast<T*>(p.o) + row.index * D;
-#pragma unroll
-    for (int dt = 0; dt < G::DT; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4)
-        store4(dst + 32 * dt + key_of(r, half), make_float4(run.o[dt][r] * inv, run.o[dt][r + 1] * inv,
-                                                            run.o[dt][r + 2] * inv, run.o[dt][r + 3] * inv));
+    store_row<T, D>(static_cast<T*>(p.o) + row.index * D, run.o, inv, half);
     if (half == 0) p.lse[row.index] = (run.m + __log2f(l)) * 0.693147180559945309f;
   } else {
     const int64_t part = (int64_t)split * p.s.num_tokens * p.q_heads + row.index;

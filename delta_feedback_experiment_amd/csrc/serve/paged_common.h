@@ -44,23 +44,20 @@ struct SeqSpan {
 
 __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
+// n <= num_seqs; num_seqs itself stands for the tokens past the last sequence,
+// which have no positions.  Its loads are asked for together.
 __device__ __forceinline__ SeqSpan seq_span(const PagedSeqs& s, int n) {
-  SeqSpan r;
-  if (s.cu) {
-    r.first = n == 0 ? 0 : clamp_int(s.cu[n], 0, s.num_tokens);
-    if (n == s.num_seqs) {  // tokens past the last sequence: no positions
-      r.count = s.num_tokens - r.first;
-      r.len = 0;
-      return r;
-    }
-    r.count = clamp_int(s.cu[n + 1], r.first, s.num_tokens) - r.first;
-  } else {
-    r.first = n;
-    r.count = 1;
+  if (!s.cu) {
+    const int64_t cap = (int64_t)s.max_pages * s.page_size;
+    return {n, 1, (int)max((int64_t)0, min((int64_t)s.lens[n], cap))};
   }
-  const int64_t cap = (int64_t)s.max_pages * s.page_size;
-  const int len = s.lens[n];
-  r.len = len < 0 ? 0 : (len > cap ? (int)cap : len);
+  if (s.num_seqs == 0) return {0, s.num_tokens, 0};
+  const int m = min(n, s.num_seqs - 1);
+  const int begin = s.cu[n], end = s.cu[m + 1], len = s.lens[m];
+  SeqSpan r;
+  r.first = n == 0 ? 0 : clamp_int(begin, 0, s.num_tokens);
+  r.count = (n == s.num_seqs ? s.num_tokens : clamp_int(end, r.first, s.num_tokens)) - r.first;
+  r.len = n == s.num_seqs ? 0 : (int)max((int64_t)0, min((int64_t)len, (int64_t)s.max_pages * s.page_size));
   return r;
 }
 
