@@ -178,8 +178,8 @@ def paged_append_(
     if check_pages:
         validate_pages(page_table, seq_lens, cu_seqlens, k.shape[0], k_pages.shape[0], k_pages.shape[1],
                        appended=True)
-    out = _registry.call(append_op, k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, cos, sin,
-                         bool(interleaved))
+    out = _registry.launch(append_op, k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, cos, sin,
+                           bool(interleaved))
     return None if q is None else out
 
 
@@ -256,8 +256,8 @@ def paged_attention(
     if check_pages:
         validate_pages(page_table, seq_lens, cu_seqlens, q.shape[0], k_pages.shape[0], k_pages.shape[1],
                        appended=False)
-    return _registry.call(attention_op, q, k_pages, v_pages, page_table, seq_lens, cu_seqlens,
-                          q.shape[2] ** -0.5 if scale is None else float(scale))
+    return _registry.launch(attention_op, q, k_pages, v_pages, page_table, seq_lens, cu_seqlens,
+                            q.shape[2] ** -0.5 if scale is None else float(scale))
 
 
 @_registry.device_op(

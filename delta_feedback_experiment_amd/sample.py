@@ -60,7 +60,7 @@ def sample_tokens(
     settings = (_setting("temperature", temperature, 1.0, rows, torch.float32),
                 _setting("top_k", top_k, 0, rows, torch.int32), _setting("top_p", top_p, 1.0, rows, torch.float32),
                 _setting("min_p", min_p, 0.0, rows, torch.float32))
-    return _registry.call(sample_op, logits, noise, *(s[0] for s in settings), *(s[1] for s in settings))
+    return _registry.launch(sample_op, logits, noise, *(s[0] for s in settings), *(s[1] for s in settings))
 
 
 def _rows(t: Tensor) -> Tensor:

@@ -404,3 +404,44 @@ def test_chunks_then_tokens_equal_one_prompt(dev):
 
     whole = run([L])
     assert rel_l2(run([64, 33, 40] + [1] * 13), whole) < 2 * TOL[torch.float32]
+
+
+def test_modes_and_profilers_see_the_operators(dev):
+    """Called past the dispatcher when nothing watches, through it otherwise:
+    the same results, version counters raised either way."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from delta_feedback_experiment_amd import paged_append_, paged_attention, sample_tokens
+
+    print("[gpu] paged cache, dispatch", flush=True)
+    c = Cache([3, 9], [1, 1], 4, 2, 64, 8, torch.bfloat16, seed=15, cu=False)
+    table, lens, _ = c.tables(dev)
+    q, k, v = (t.to(dev) for t in (c.q, c.k, c.v))
+    logits, noise = torch.randn(2, 100, device=dev), torch.randn(2, 100, device=dev)
+
+    def run(q=q):
+        kp, vp = c.k_pages.to(dev), c.v_pages.to(dev)
+        version = kp._version
+        out = paged_append_(k, v, kp, vp, table, lens, q=q)
+        assert kp._version == vp._version == version + 1
+        return (out, kp, *paged_attention(out, kp, vp, table, lens), *sample_tokens(logits, noise))
+
+    class Watch(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen.append(func._schema.name.split("::")[-1])
+            return func(*args, **(kwargs or {}))
+
+    names = {"paged_append_", "paged_attention", "sample_tokens"}
+    plain = run()
+    with Watch() as watch:
+        watched = run()
+    assert names <= set(watch.seen)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        profiled = run()
+    assert names <= {e.name.split("::")[-1] for e in prof.events()}
+    for other in (watched, profiled, run(q.requires_grad_())):
+        assert all(torch.equal(a.detach().nan_to_num(9), b.nan_to_num(9)) for a, b in zip(other, plain))
