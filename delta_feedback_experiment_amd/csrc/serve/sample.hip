@@ -203,7 +203,7 @@ struct Lds {
     float hist[kBins + 2][kThreads];
     struct {
       uint32_t candidates[kCandidates];  // indices
-      float few[kFewBins + 2][kThreads];
+      uint32_t few[kFewBins + 2][kThreads];
     };
   };
   uint64_t list[kList];
@@ -582,9 +582,23 @@ __device__ __forceinline__ Ending find_ending(const RowData<T>& row, const Scale
     // The column is the thread's own: read, add, write.  (LDS additions without a
     // return take 176 cycles a wave here.)  Two logits at a time over the row, so
     // that two reads are on their way.
-    float* column = e.gathered ? &lds.few[0][threadIdx.x] : &lds.hist[0][threadIdx.x];
-    for (int i = 0; i < b.n + 2; ++i) column[i * kThreads] = 0.f;
-    const auto put = [&](int i, float w) { column[i * kThreads] += w; };
+    // A list's order differs from run to run, so its weights are added as whole
+    // numbers, of 2^-26 of the interval's largest (27 a thread at most), and what
+    // is above the interval is known already.
+    float* column = &lds.hist[0][threadIdx.x];
+    uint32_t* few_column = &lds.few[0][threadIdx.x];
+    int units = 0;  // a weight's, as a power of two
+    if (e.gathered) {
+      if (mass) units = min(26 - __builtin_amdgcn_frexp_expf(s.weight(b.most)), 126);
+      for (int i = 0; i < b.n + 2; ++i) few_column[i * kThreads] = 0;
+    } else {
+      for (int i = 0; i < b.n + 2; ++i) column[i * kThreads] = 0.f;
+    }
+    const float unit = ldexpf(1.f, units);
+    const auto put = [&](int i, float w) {
+      if (!e.gathered) column[i * kThreads] += w;
+      else if (i > 0) few_column[i * kThreads] += (uint32_t)(w * unit);
+    };
     const auto put2 = [&](int i, float u, int j, float w) {
       const float a = column[i * kThreads], c = column[j * kThreads];
       column[i * kThreads] = a + u;
@@ -606,13 +620,13 @@ __device__ __forceinline__ Ending find_ending(const RowData<T>& row, const Scale
     __syncthreads();
     // the rows' sums, a few a wave
     for (int q = threadIdx.x >> 6; q < b.n + 2; q += kWaves) {
-      const float* r = (e.gathered ? lds.few[0] : lds.hist[0]) + q * kThreads;
       double t = 0.;
 #pragma unroll
-      for (int i = 0; i < kThreads / 64; ++i) t += r[i * 64 + lane];
+      for (int i = 0; i < kThreads / 64; ++i)
+        t += e.gathered ? (double)lds.few[q][i * 64 + lane] : (double)lds.hist[q][i * 64 + lane];
 #pragma unroll
       for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o);
-      if (lane == 0) lds.bins[q] = t;
+      if (lane == 0) lds.bins[q] = ldexp(t, -units);
     }
     __syncthreads();
     // every wave for itself, a lane a row: what the rows up to it hold
@@ -623,6 +637,7 @@ __device__ __forceinline__ Ending find_ending(const RowData<T>& row, const Scale
       const double y = __shfl_up(upto, o);
       if (lane >= o) upto += y;
     }
+    if (e.gathered) upto += e.before;
     if (round == 0) {
       const double total = __shfl(upto, 63);
       if (mass) e.goal *= total;

@@ -204,3 +204,22 @@ def test_draws_follow_the_distribution(dev):
     p[kept] = torch.softmax(z, 0)
     freq = torch.bincount(token.long().cpu(), minlength=V).double() / n
     assert ((freq - p).abs() <= 5 * (p * (1 - p) / n).sqrt()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_lists_in_any_order(dev, dtype):
+    """Prefixes of a few thousand near-equal tokens, which a list holds in
+    whatever order it was filled: the same token every time, the oracle's."""
+    from delta_feedback_experiment_amd import sample_tokens
+
+    print(f"[gpu] sample, lists {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(15)
+    logits = (0.05 * torch.randn(48, 20011, generator=gen)).to(dtype)
+    logits[:, :4000] += 4
+    noise = gumbel(48, 20011, seed=16)
+    settings = [{"top_p": 0.05 + 0.9 * r / 48, "temperature": 0.5 + r % 3} for r in range(48)]
+    want = check(dev, logits, noise, settings)
+    t, p = (torch.tensor([s[n] for s in settings], device=dev) for n in ("temperature", "top_p"))
+    x, g = logits.to(dev), noise.to(dev)
+    for _ in range(10):
+        assert torch.equal(sample_tokens(x, g, temperature=t, top_p=p)[0], want)
