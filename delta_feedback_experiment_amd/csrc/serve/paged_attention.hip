@@ -18,13 +18,27 @@
 // half of a row is operand i of the lane's half (BF16: one 32x32x16 step; FP32:
 // four 32x32x2 steps).
 //
-// Two forms, in one launch.  Up to 32 rows of a tile (decode): four waves take 32 keys each
-// in turn, each with its own m, l and O, and join at the end; keys go straight
-// from memory to operand registers, values through a wave's own piece of LDS
-// (the transposing reads), the next tile's loads in flight during a tile's
-// arithmetic.  More rows (a chunk): four waves of 32 rows share tiles of 64 keys
-// staged in LDS, double-buffered.  Where rows are few, a sequence's keys are
-// split over workgroups and a second kernel joins the parts.
+// Two forms, in one launch.  Up to 32 rows of a sequence (decode, a few proposed
+// tokens): four waves take 32 keys each in turn, each with its own m, l and O,
+// and join at the end; keys go straight from memory to operand registers, values
+// through a wave's own piece of LDS (the transposing reads), the next tile's
+// loads in flight during a tile's arithmetic.  More rows (a chunk): four waves of
+// 32 rows share tiles of 64 keys staged in LDS, double-buffered.  Where rows are
+// few, a sequence's keys are split over workgroups and a second kernel joins the
+// parts.
+//
+// Roundings to BF16: the probabilities, as the second product's operand (their
+// sum l is of the unrounded ones), and the output; scores, m, l and O are FP32.
+//
+// What bounds it, measured in BF16 with heads of 128 (a large read runs at 4.0 to
+// 5.0 TB/s, a large matrix product at 1188 TFLOP/s).  Decode, 256 sequences of
+// 2,600 keys, 32/8 heads: 546 us, 4.98 TB/s of keys and values.  One sequence of
+// 131,072 keys: 114 us, 4.7 TB/s.  2,048 tokens after 14,336, 32/8 heads: 602 us,
+// 855 TFLOP/s: a tile's 32 products of 16 ns a wave run beside the other
+// workgroup's softmax, whose 64 exponentials and about 400 other operations a
+// lane take as long; the two do not overlap fully.  13 prompts of 250 to 1,659
+// tokens, 16/4 heads: 87 us, 587 TFLOP/s: 6 us of a row tile's 33 are its way to
+// its first keys and its output.
 #include <math.h>
 
 #include "paged_common.h"
@@ -246,7 +260,9 @@ __device__ __forceinline__ int wave_sum(int x) {
 // with the most keys first: lane n has sequence n (fewer than 64).  A tile's
 // level is its last row counted from the sequence's first position, in tiles;
 // a sequence has one tile a level from lo up, so the tiles from a level up are
-// counted by one sum over the wave, and the level of the t-th by bisection.
+// counted by one sum over the wave, and the level of the t-th by bisection.  In
+// the sequences' order instead the last long ones begin when the rest is nearly
+// done: 13 prompts of 250 to 1,659 tokens 110 us, so 93.
 template <int M>
 __device__ __forceinline__ bool find_longest(const AttnParams& p, int t, Tile& tile) {
   const int lane = threadIdx.x & 63;
@@ -606,7 +622,8 @@ constexpr int kKeyTile = 64;
 
 // WHOLE: the rows that a wave stages at a time, 64 / NC keys, lie in one page
 // (the page size is a multiple of them): a load's address is the page's, in
-// scalar registers, and a lane's constant part.
+// scalar registers, and a lane's constant part.  2,048 tokens after 14,336:
+// 602 us, with every lane's own addresses 648; 13 prompts: 87 and 92.
 template <typename T, int D> struct RowsLds {
   __align__(16) char kv[4 * kKeyTile * Geo<T, D>::RB];  // two stages of K, V
   // of tile t % 3: its keys with values that are not finite, and those without a page
@@ -897,22 +914,31 @@ struct Plan {
 
 // Which form takes which sequences, and into how many splits a sequence's keys
 // are cut at most, from what the host knows: sequences have num_tokens /
-// num_seqs tokens each.
+// num_seqs tokens each.  Times are BF16, heads of 128, unless they say more.
 Plan plan(AttnParams& p) {
   const int64_t group = p.group.d, N = p.s.num_tokens, S = p.s.num_seqs, heads = p.kv_heads;
   const bool packed = p.s.cu != nullptr;
   Plan r;
+  // More than 32 rows a sequence go to 128-row tiles: 13 prompts take 87 us so,
+  // and 239 as tiles of 32 rows; 64 sequences of 40 rows after 1,900 keys 81 and
+  // 103.  Not where those tiles leave the card half empty: one prompt of 1,531
+  // tokens, 8/2 heads, is 98 of them (49 us) or 386 of 32 rows (36 us).
   p.key_rows = 32;
   r.row_tiles = packed ? tile_bound(N, S, group, kRowTile, true) : 0;
   if (packed && r.row_tiles * heads < kSlots / 2) p.key_rows = INT32_MAX;
   if (p.key_rows != 32) r.row_tiles = 0;
   r.key_tiles = packed && p.key_rows == 32 ? S + 1 : tile_bound(N, S, group, 32, packed);
-  // a row's part of a split costs 2 D floats, a key 2 D numbers a tile: enough
-  // keys a split that the parts stay a small share
+  // A row's part of a split costs 2 D floats, a key 2 D numbers a tile: enough
+  // keys a split that the parts stay a small share.  8 keys a row of the tile:
+  // the 64 sequences of 40 rows take 81 us, with 16 they take 83.
   const int64_t per_seq = S > 0 ? (N * group + S - 1) / S : 1;
   const int64_t tile_rows = per_seq < 32 || p.key_rows != 32 ? (per_seq < 32 ? per_seq : 32)
                                                              : (per_seq < kRowTile ? per_seq : kRowTile);
   p.min_chunk = (int)((8 * tile_rows + kMinChunk - 1) / kMinChunk * kMinChunk);
+  // Four times the workgroups the card holds where a sequence has less than a
+  // full tile, since lengths differ and the longest decides: the same 64
+  // sequences take 81 us with four, 89 with two, 127 with one.  Full tiles once:
+  // their parts are many.
   const int64_t items = (packed && p.key_rows == 32 ? r.row_tiles + (per_seq <= 32 ? S : 0) : r.key_tiles) * heads;
   const int64_t cap = ((int64_t)p.s.max_pages * p.s.page_size + p.min_chunk - 1) / p.min_chunk;
   int64_t want = kSlots * (per_seq < kRowTile ? 4 : 1) / (items > 0 ? items : 1);
@@ -940,6 +966,9 @@ int launch_attention(AttnParams p, hipStream_t s) {
     hipLaunchKernelGGL((paged_attention_kernel<T, D, false>), grid, block, 0, s, p);
   if (int st = launch_status("pkda_paged_attention")) return st;
   if (p.splits == 1) return 0;
+  // A row's parts over four waves while rows are too few to fill the card: one
+  // token after 131,071, 32 rows of 256 parts, 114 us against 120 in all; with
+  // 10,240 rows of up to 10 parts one wave a row, 81 us against 95.
   if (rows < 2 * kSlots)
     hipLaunchKernelGGL((paged_attention_join_kernel<T, D, kWaves>), dim3((unsigned)rows), block, 0, s, p);
   else
