@@ -23,7 +23,15 @@
 // indices.
 //
 // Scores z + noise are those of the definition, z correctly rounded, so that the
-// token does not depend on the path.  Sums over bins and lists are FP64.
+// token does not depend on the path.  A thread's own sums are FP32, or whole
+// numbers over lists, whose order varies; sums over threads and bins are FP64.
+//
+// Measured, BF16, 256 rows of 131,072 normal logits times 3 (a row a compute
+// unit; 67 MB read once are 17 us, with all the noise 42): greedy 17 us, top-k 50
+// 29, top-k 200 and top-p 0.9 35, min-p 0.05 27, no filter 45, top-p 0.5 56, 0.9
+// 91, 0.99 108, top-k 5000 97; 4 rows of 50,304: 9 to 56.  What is left of a
+// top-p row is one exponential and one column addition a logit, then some 20
+// block-wide steps one after another.
 #include "pkda_common.h"
 #include "serve/pkda_serve_gfx950.h"
 
@@ -32,9 +40,9 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kList = 1024;         // tokens of a sorted list: one a thread
-constexpr int kBins = 32, kFewBins = 8;  // of a round over the row, over a list
-constexpr int kCandidates = 27136;       // tokens of an unsorted list
+constexpr int kList = 1024;              // tokens of a sorted list: one a thread
+constexpr int kBins = 32, kFewBins = 8;  // of a round over the row, over a list: what LDS has room for
+constexpr int kCandidates = 27136;       // tokens of an unsorted list: likewise
 constexpr float kMaxFloat = 3.402823466e38f;
 constexpr uint32_t kMinKey = 0x00800000u;  // the key of -kMaxFloat
 
