@@ -71,6 +71,7 @@ struct AttnParams {
   bool negate;   // scale < 0: queries are negated
   int splits;
   int min_chunk;       // keys of a split, at least
+  int whole;           // sequences of up to so many positions are not split
   int key_rows;        // sequences of up to so many rows run with their keys over the waves
   unsigned row_blocks; // workgroups of the others, before those
   void* o;
@@ -186,6 +187,7 @@ struct Tile {
 };
 
 __device__ __forceinline__ int split_chunk(const AttnParams& p, int len) {
+  if (len <= p.whole) return p.whole;
   const int c = (len + p.splits - 1) / p.splits;
   return max(p.min_chunk, (c + kMinChunk - 1) / kMinChunk * kMinChunk);
 }
@@ -941,7 +943,14 @@ Plan plan(AttnParams& p) {
   // their parts are many.
   const int64_t items = (packed && p.key_rows == 32 ? r.row_tiles + (per_seq <= 32 ? S : 0) : r.key_tiles) * heads;
   const int64_t cap = ((int64_t)p.s.max_pages * p.s.page_size + p.min_chunk - 1) / p.min_chunk;
+  // Where the sequences fill the card by themselves, the short ones stay whole, and
+  // all do where none can be long: 64 around 500 keys, 8 heads, take 29 us, and 38
+  // in pieces; 128 around 1,000 120 and 126.  Longer ones differ by more than the
+  // card evens out: 64 around 4,000, up to 7,500, 218 in four pieces and 296 whole
+  // (228 with those up to 2,048 whole, 219 with those up to 1,024).
+  p.whole = items >= kSlots ? 1024 : 0;
   int64_t want = kSlots * (per_seq < kRowTile ? 4 : 1) / (items > 0 ? items : 1);
+  if ((int64_t)p.s.max_pages * p.s.page_size <= 2 * p.whole) want = 1;
   if (want > cap) want = cap;
   if (want > kMaxSplits) want = kMaxSplits;
   p.splits = want < 1 ? 1 : (int)want;

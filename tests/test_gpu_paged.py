@@ -445,3 +445,19 @@ def test_modes_and_profilers_see_the_operators(dev):
     assert names <= {e.name.split("::")[-1] for e in prof.events()}
     for other in (watched, profiled, run(q.requires_grad_())):
         assert all(torch.equal(a.detach().nan_to_num(9), b.nan_to_num(9)) for a, b in zip(other, plain))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_full_card_splits_long_sequences_only(dev, dtype):
+    """512 (sequence, head) pairs: those of up to 1,024 positions stay whole, the
+    others are split; none where the table holds no more than 2,048."""
+    print(f"[gpu] paged attention, whole and split {dtype}", flush=True)
+    for lens in ([1024, 1025, 2600, 7], [1024, 1500, 2000, 0]):
+        c = Cache(lens, [1] * 4, 128, 128, 32, 16, dtype, seed=17, cu=False, tail_pages=1)
+        o, lse = c.attend(dev)
+        cu = torch.arange(5, dtype=torch.int32)
+        ro, rl = oracle.attention_of_sequences(c.q, c.k_pages, c.v_pages, c.table, c.lens, cu)
+        assert rel_l2(o.float(), ro) < TOL[dtype]
+        some = c.lens > 0
+        gap = (lse.cpu().double() - rl).abs() / (1 + rl.abs())
+        assert float(gap[some].max()) < 1e-5 and torch.isneginf(lse.cpu()[~some]).all()
