@@ -84,8 +84,10 @@ def _check_cache(name: str, x: Tensor, k_pages: Tensor, v_pages: Tensor, page_ta
 
 
 def _aligned(t: Tensor, stride: int) -> bool:
-    # fake tensors have no address: the offset is what a view adds to its storage
-    return (stride | t.storage_offset()) * t.element_size() % 16 == 0
+    # fake tensors have no address: the offset is what a view adds to its storage (a
+    # compiler's trace has no offset either; the launch checks the address)
+    offset = 0 if torch.compiler.is_compiling() else t.storage_offset()
+    return (stride | offset) * t.element_size() % 16 == 0
 
 
 def _rows(t: Tensor) -> Tensor:
