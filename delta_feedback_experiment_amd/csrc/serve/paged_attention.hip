@@ -1001,7 +1001,7 @@ int attention_sizes(const pkda_paged_attention_args* a, AttnParams& p) {
   p.q_heads = a->q_heads;
   p.kv_heads = a->kv_heads;
   p.group = FastDiv::make((uint32_t)(a->q_heads / a->kv_heads));
-  PKDA_REQUIRE((int64_t)a->num_tokens * p.group.d <= INT32_MAX, PKDA_EINVAL, "%d tokens of %d heads", a->num_tokens,
+  PKDA_REQUIRE((int64_t)a->num_tokens * p.group.d <= 1 << 30, PKDA_EINVAL, "%d tokens of %d heads", a->num_tokens,
                a->q_heads);
   plan(p);
   return 0;

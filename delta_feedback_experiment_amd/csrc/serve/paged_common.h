@@ -108,7 +108,9 @@ int paged_seqs_from(const A* a, PagedSeqs& s) {
   PKDA_REQUIRE(a->num_seqs >= 0 && a->num_tokens >= 0, PKDA_EINVAL, "num_seqs %d, num_tokens %d", a->num_seqs,
                a->num_tokens);
   PKDA_REQUIRE(a->kv_heads >= 1 && a->kv_heads <= 65535, PKDA_EINVAL, "kv_heads %d", a->kv_heads);
-  PKDA_REQUIRE(a->page_size >= 1 && a->max_pages >= 0 && (int64_t)a->page_size * a->max_pages <= INT32_MAX,
+  // positions and a sequence's rows stay far enough under 2^31 that a tile past
+  // the last one is still a number
+  PKDA_REQUIRE(a->page_size >= 1 && a->max_pages >= 0 && (int64_t)a->page_size * a->max_pages <= 1 << 30,
                PKDA_EINVAL, "page_size %d x %d pages of a table row", a->page_size, a->max_pages);
   PKDA_REQUIRE(a->num_pages >= 0 && a->num_pages <= INT32_MAX, PKDA_EINVAL, "num_pages");
   s.cu = a->cu_seqlens; s.lens = a->seq_lens; s.table = a->page_table;

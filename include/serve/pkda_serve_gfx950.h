@@ -56,7 +56,7 @@ typedef struct pkda_paged_append_args {
   int32_t struct_size;  /* sizeof(pkda_paged_append_args) */
   int32_t dtype;        /* pkda_dtype of q, k, v, the pools */
   int32_t num_seqs, num_tokens, q_heads, kv_heads, head_dim; /* q_heads 0: no q */
-  int32_t page_size, max_pages; /* max_pages: pages of a table row */
+  int32_t page_size, max_pages; /* max_pages: pages of a table row; page_size * max_pages <= 2^30 */
   int64_t num_pages;
   int64_t table_stride;         /* elements between table rows */
   const int32_t* cu_seqlens;    /* [num_seqs + 1] or NULL (num_tokens == num_seqs) */

@@ -461,3 +461,34 @@ def test_a_full_card_splits_long_sequences_only(dev, dtype):
         some = c.lens > 0
         gap = (lse.cpu().double() - rl).abs() / (1 + rl.abs())
         assert float(gap[some].max()) < 1e-5 and torch.isneginf(lse.cpu()[~some]).all()
+
+
+def test_opcheck_and_compile(dev):
+    """The schemas' marks match what the kernels write, the fake forms agree in
+    shape and dtype, and a compiled step gives the eager bits."""
+    from delta_feedback_experiment_amd import paged_append_, paged_attention, sample_tokens
+
+    print("[gpu] paged cache, opcheck and compile", flush=True)
+    c = Cache([3, 9, 20], [2, 1, 20], 4, 2, 64, 8, torch.bfloat16, seed=18)
+    table, lens, cu = c.tables(dev)
+    q, k, v, kp, vp = (t.to(dev) for t in (c.q, c.k, c.v, c.k_pages.nan_to_num(0.5), c.v_pages.nan_to_num(0.5)))
+    angle = torch.rand(table.shape[1] * 8, 32, device=dev)
+    logits, noise = torch.randn(3, 100, device=dev), torch.randn(3, 100, device=dev)
+    ops, utils = torch.ops.pkda_mi355x, ("test_schema", "test_faketensor")
+    for query in (q, None):
+        torch.library.opcheck(ops.paged_append_.default,
+                              (k, v, kp, vp, table, lens, cu, query, angle.cos(), angle.sin(), False), test_utils=utils)
+    torch.library.opcheck(ops.paged_attention.default, (q, kp, vp, table, lens, cu, 0.125), test_utils=utils)
+    torch.library.opcheck(ops.sample_tokens.default, (logits, noise, None, None, None, None, 0.7, 5, 0.9, 0.01),
+                          test_utils=utils)
+
+    def step(q, k, v, kp, vp):
+        q = paged_append_(k, v, kp, vp, table, lens, cu_seqlens=cu, q=q, cos=angle.cos(), sin=angle.sin())
+        o, lse = paged_attention(q * 1.0, kp, vp, table, lens, cu_seqlens=cu)
+        return (o, lse, *sample_tokens(logits + o.float().mean() * 0, noise, top_k=5))
+
+    pools = [(kp.clone(), vp.clone()) for _ in range(2)]
+    eager = step(q, k, v, *pools[0])
+    compiled = torch.compile(step, fullgraph=True, backend="aot_eager")(q, k, v, *pools[1])
+    for a, b in zip((*eager, *pools[0]), (*compiled, *pools[1])):
+        assert torch.equal(a, b)

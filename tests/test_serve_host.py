@@ -70,6 +70,17 @@ def test_more_refusals_before_any_launch():
             _lib.call("pkda_sample", args, 0)
 
 
+@pytest.mark.parametrize("kw,match", [
+    (dict(page_size=2 ** 20, max_pages=2 ** 10 + 1), "page_size"), (dict(page_size=2 ** 31 - 1, max_pages=1), "page_size"),
+    (dict(num_tokens=2 ** 29 + 1, cu_seqlens=16), "tokens of")])
+def test_positions_and_rows_stay_clear_of_32_bits(kw, match):
+    """The kernels add up to a tile to a position or a row: none may wrap."""
+    from delta_feedback_experiment_amd import _lib
+
+    with pytest.raises(ValueError, match=match):
+        _lib.call("pkda_paged_attention", _paged(_lib.PagedAttentionArgs, o=96, lse=112, **kw), 0)
+
+
 def test_operators_refuse_cpu_tensors():
     from delta_feedback_experiment_amd import paged_append_, paged_attention, sample_tokens
 
