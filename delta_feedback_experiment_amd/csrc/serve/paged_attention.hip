@@ -34,11 +34,12 @@
 // 5.0 TB/s, a large matrix product at 1188 TFLOP/s).  Decode, 256 sequences of
 // 2,600 keys, 32/8 heads: 546 us, 4.98 TB/s of keys and values.  One sequence of
 // 131,072 keys: 114 us, 4.7 TB/s.  2,048 tokens after 14,336, 32/8 heads: 602 us,
-// 855 TFLOP/s: a tile's 32 products of 16 ns a wave run beside the other
-// workgroup's softmax, whose 64 exponentials and about 400 other operations a
-// lane take as long; the two do not overlap fully.  13 prompts of 250 to 1,659
-// tokens, 16/4 heads: 87 us, 587 TFLOP/s: 6 us of a row tile's 33 are its way to
-// its first keys and its output.
+// 855 TFLOP/s: a wave's 32 products a tile are 1,024 cycles, its 246 vector
+// instructions, 32 exponentials among them, about 1,370, and its reads of LDS
+// about 800; the other workgroup's wave on the SIMD overlaps them only in part
+// (2,500 cycles a tile and wave).  13 prompts of 250 to 1,659 tokens, 16/4 heads:
+// 87 us, 587 TFLOP/s: 6 us of a row tile's 33 are its way to its first keys and
+// its output.
 #include <math.h>
 
 #include "paged_common.h"
