@@ -33,12 +33,12 @@
 // What bounds it, measured in BF16 with heads of 128 (a large read runs at 4.0 to
 // 5.0 TB/s, a large matrix product at 1188 TFLOP/s).  Decode, 256 sequences of
 // 2,600 keys, 32/8 heads: 546 us, 4.98 TB/s of keys and values.  One sequence of
-// 131,072 keys: 114 us, 4.7 TB/s.  2,048 tokens after 14,336, 32/8 heads: 602 us,
-// 855 TFLOP/s: a wave's 32 products a tile are 1,024 cycles, its 246 vector
+// 131,072 keys: 114 us, 4.7 TB/s.  2,048 tokens after 14,336, 32/8 heads: 585 us,
+// 880 TFLOP/s: a wave's 32 products a tile are 1,024 cycles, its 246 vector
 // instructions, 32 exponentials among them, about 1,370, and its reads of LDS
 // about 800; the other workgroup's wave on the SIMD overlaps them only in part
-// (2,500 cycles a tile and wave).  13 prompts of 250 to 1,659 tokens, 16/4 heads:
-// 87 us, 587 TFLOP/s: 6 us of a row tile's 33 are its way to its first keys and
+// (2,400 cycles a tile and wave).  13 prompts of 250 to 1,659 tokens, 16/4 heads:
+// 84 us, 606 TFLOP/s: 6 us of a row tile's 33 are its way to its first keys and
 // its output.
 #include <math.h>
 
@@ -334,9 +334,14 @@ __device__ __forceinline__ void arrived(u32x4 (&q)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(q[i]));
 }
 
-// A row's softmax while its keys pass.
+// A row's softmax while its keys pass.  m is a maximum of the keys so far, or less
+// by up to kSlack (probabilities are then at most 2^kSlack; nothing is lost by it):
+// with the exact one some row of the 32 raises it, and all of a tile's outputs are
+// rescaled, in nearly every tile of the first fifty (2,048 tokens after 14,336 605
+// us, so 585; 13 prompts 88 and 84).
+constexpr float kSlack = 8.f;
 template <int DT> struct Running {
-  float m, l;  // maximum (base 2), and the sum over this half's keys
+  float m, l;  // m (base 2), and the sum over this half's keys
   f32x16 o[DT];
   __device__ __forceinline__ void init() {
     m = -INFINITY;
@@ -355,8 +360,10 @@ template <int DT> struct Running {
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     mx = join_halves(mx, [](float a, float b) { return fmaxf(a, b); }) * scale2;
-    if (__any(mx > m)) {
-      const float mn = fmaxf(m, mx);
+    // the maximum is followed only where it has grown by more than kSlack
+    const bool grown = mx > m + kSlack;
+    if (__any(grown)) {
+      const float mn = grown ? mx : m;
       const float a = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
       m = mn;
       l *= a;
