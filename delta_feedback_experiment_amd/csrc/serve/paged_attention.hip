@@ -6,7 +6,8 @@
 // any number.  Scores, softmax and output run in one pass over the keys with
 // the row's running maximum m and sum l (base 2, FP32):
 //   m' = max(m, max_s S),  p = 2^(S - m'),  l = l 2^(m - m') + sum_s p,
-//   O = O 2^(m - m') + p V,   o = O / l,  lse = (m + log2 l) ln 2.
+//   O = O 2^(m - m') + p V,   o = O / l,  lse = (m + log2 l) ln 2,
+// which hold for any m; it stays near the maximum (kSlack below).
 //
 // Products.  Both are taken transposed, S^T = K Q^T and O^T = V^T P^T, as
 // 32x32 MFMA tiles.  A lane then holds one query row (its column) and 16 of a
