@@ -336,10 +336,13 @@ __device__ __forceinline__ void arrived(u32x4 (&q)[N]) {
 }
 
 // A row's softmax while its keys pass.  m is a maximum of the keys so far, or less
-// by up to kSlack (probabilities are then at most 2^kSlack; nothing is lost by it):
-// with the exact one some row of the 32 raises it, and all of a tile's outputs are
-// rescaled, in nearly every tile of the first fifty (2,048 tokens after 14,336 605
-// us, so 585; 13 prompts 88 and 84).
+// by up to `slack` (probabilities are then at most 2^slack).  With the exact one
+// some row of a wave raises it, and all of a tile's outputs are rescaled, in nearly
+// every tile of the first fifty: 2,048 tokens after 14,336 605 us, and 585 with a
+// slack of 8; 13 prompts 88 and 84.  But the largest probability is then no longer
+// 1, which BF16 holds exactly: the output's error against 64 bits is 0.0023 of its
+// size, and 0.0020 with the exact maximum (0.0017 is the output's own rounding).
+// Few rows (up to half a tile of 128), which wait for memory, keep the exact one.
 constexpr float kSlack = 8.f;
 template <int DT> struct Running {
   float m, l;  // m (base 2), and the sum over this half's keys
@@ -354,15 +357,14 @@ template <int DT> struct Running {
   }
   // scores of N tiles of keys -> their probabilities
   template <int N>
-  __device__ __forceinline__ void step(f32x16 (&s)[N], float scale2) {
+  __device__ __forceinline__ void step(f32x16 (&s)[N], float scale2, float slack) {
     float mx = s[0][0];
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     mx = join_halves(mx, [](float a, float b) { return fmaxf(a, b); }) * scale2;
-    // the maximum is followed only where it has grown by more than kSlack
-    const bool grown = mx > m + kSlack;
+    const bool grown = mx > m + slack;
     if (__any(grown)) {
       const float mn = grown ? mx : m;
       const float a = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
@@ -567,7 +569,7 @@ __device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block,
         if (key0 + i > row.pos || !((there >> i) & 1)) s[0][r] = -INFINITY;
       }
     }
-    run.step(s, p.scale2);
+    run.step(s, p.scale2, 0.f);
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     mma_values<T, D>(run.o, sv, 0, s[0], lane);
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
@@ -806,7 +808,7 @@ __device__ __forceinline__ void attend_rows(const AttnParams& p, unsigned block,
           for (int r = 0; r < 16; ++r)
             if (((n ? gone1 : gone0) >> key_of(r, half)) & 1) s[n][r] = -INFINITY;
       }
-      run.step(s, p.scale2);
+      run.step(s, p.scale2, tile.rows > kRowTile / 2 ? kSlack : 0.f);
 #pragma unroll
       for (int n = 0; n < 2; ++n) mma_values<T, D>(run.o, sk + kTileBytes, 32 * n, s[n], lane);
       const uint64_t bad = __builtin_amdgcn_readfirstlane(odd.x) |
