@@ -266,7 +266,7 @@ __device__ __forceinline__ int wave_sum(int x) {
 // a sequence has one tile a level from lo up, so the tiles from a level up are
 // counted by one sum over the wave, and the level of the t-th by bisection.  In
 // the sequences' order instead the last long ones begin when the rest is nearly
-// done: 13 prompts of 250 to 1,659 tokens 110 us, so 93.
+// done: 13 prompts of 250 to 1,659 tokens 99 us, so 84.
 template <int M>
 __device__ __forceinline__ bool find_longest(const AttnParams& p, int t, Tile& tile) {
   const int lane = threadIdx.x & 63;
@@ -338,8 +338,8 @@ __device__ __forceinline__ void arrived(u32x4 (&q)[N]) {
 // A row's softmax while its keys pass.  m is a maximum of the keys so far, or less
 // by up to `slack` (probabilities are then at most 2^slack).  With the exact one
 // some row of a wave raises it, and all of a tile's outputs are rescaled, in nearly
-// every tile of the first fifty: 2,048 tokens after 14,336 605 us, and 585 with a
-// slack of 8; 13 prompts 88 and 84.  But the largest probability is then no longer
+// every tile of the first fifty: 2,048 tokens after 14,336 599 us, and 585 with a
+// slack of 8; 13 prompts 87 and 84.  But the largest probability is then no longer
 // 1, which BF16 holds exactly: the output's error against 64 bits is 0.0023 of its
 // size, and 0.0020 with the exact maximum (0.0017 is the output's own rounding).
 // Few rows (up to half a tile of 128), which wait for memory, keep the exact one.
@@ -636,7 +636,7 @@ constexpr int kKeyTile = 64;
 // WHOLE: the rows that a wave stages at a time, 64 / NC keys, lie in one page
 // (the page size is a multiple of them): a load's address is the page's, in
 // scalar registers, and a lane's constant part.  2,048 tokens after 14,336:
-// 602 us, with every lane's own addresses 648; 13 prompts: 87 and 92.
+// 585 us, with every lane's own addresses 626; 13 prompts: 84 and 88.
 template <typename T, int D> struct RowsLds {
   __align__(16) char kv[4 * kKeyTile * Geo<T, D>::RB];  // two stages of K, V
   // of tile t % 3: its keys with values that are not finite, and those without a page
@@ -932,10 +932,10 @@ Plan plan(AttnParams& p) {
   const int64_t group = p.group.d, N = p.s.num_tokens, S = p.s.num_seqs, heads = p.kv_heads;
   const bool packed = p.s.cu != nullptr;
   Plan r;
-  // More than 32 rows a sequence go to 128-row tiles: 13 prompts take 87 us so,
-  // and 239 as tiles of 32 rows; 64 sequences of 40 rows after 1,900 keys 81 and
-  // 103.  Not where those tiles leave the card half empty: one prompt of 1,531
-  // tokens, 8/2 heads, is 98 of them (49 us) or 386 of 32 rows (36 us).
+  // More than 32 rows a sequence go to 128-row tiles: 13 prompts take 84 us so,
+  // and 238 as tiles of 32 rows; 64 sequences of 40 rows after 1,900 keys 81 and
+  // 101.  Not where those tiles leave the card half empty: one prompt of 1,531
+  // tokens, 8/2 heads, is 98 of them (47 us) or 386 of 32 rows (36 us).
   p.key_rows = 32;
   r.row_tiles = packed ? tile_bound(N, S, group, kRowTile, true) : 0;
   if (packed && r.row_tiles * heads < kSlots / 2) p.key_rows = INT32_MAX;
