@@ -62,7 +62,9 @@ __device__ __forceinline__ SeqSpan seq_span(const PagedSeqs& s, int n) {
 }
 
 // The largest n <= num_seqs with f(n) <= x, for f non-decreasing with
-// f(0) <= x, by the whole wave, 64 candidates a step; x is wave-uniform.
+// f(0) <= x, by the whole wave, 64 candidates a step; x is wave-uniform.  Where
+// f falls (bounds that cannot be) it is some n with f(n) <= x all the same: a
+// step goes on from the last of the candidates before the first that is above.
 template <typename F>
 __device__ __forceinline__ int wave_upper(int num_seqs, int64_t x, F f) {
   const int lane = threadIdx.x & 63;
@@ -71,8 +73,8 @@ __device__ __forceinline__ int wave_upper(int num_seqs, int64_t x, F f) {
     const int step = (span + 63) / 64;
     const int i = lane * step;
     const bool below = i < span && f(base + i) <= x;
-    const int n = __popcll(__ballot(below));
-    const int at = n > 0 ? (n - 1) * step : 0;
+    const uint64_t above = ~__ballot(below);
+    const int at = (above ? __builtin_ctzll(above) - 1 : 63) * step;  // lane 0's is below
     base += at;
     span = min(step, span - at);
   }

@@ -16,9 +16,11 @@ sequence without: the decode step.  Neither records autograd history.
 
 Device data that names what does not exist stays inside the buffers: a length
 past the table's row is cut to it, ``cu_seqlens`` is clamped to the packed
-length, a page number outside the pool holds nothing, a token of no sequence
-(padding past ``cu_seqlens[-1]``) is stored nowhere and attends to nothing.
-``check_pages=True`` raises instead, at the price of a copy to the host.
+length and begins at 0, a page number outside the pool holds nothing, a token of
+no sequence (padding past ``cu_seqlens[-1]``) is stored nowhere and attends to
+nothing.  ``cu_seqlens`` that falls names no sequences: what the tokens' outputs
+and their sequences' rows then hold is undefined.  ``check_pages=True`` raises
+instead, at the price of a copy to the host.
 """
 
 from __future__ import annotations

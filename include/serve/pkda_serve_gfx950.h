@@ -14,9 +14,11 @@
  *
  * What a caller's device data can say wrong stays inside the buffers: a length
  * past the table's row is cut to it, document bounds are clamped to the packed
- * length, a page number outside the pool holds nothing (nothing is stored
- * there, its positions are masked), a token of no sequence (past cu[num_seqs],
- * or before its sequence's position 0) has no key.
+ * length and cu[0] counts as 0, a page number outside the pool holds nothing
+ * (nothing is stored there, its positions are masked), a token of no sequence
+ * (past cu[num_seqs], or before its sequence's position 0) has no key.  Bounds
+ * that fall name no sequences: which of the sequences' rows are written, and
+ * what the tokens' outputs hold, is undefined then.
  */
 #ifndef PKDA_SERVE_GFX950_H
 #define PKDA_SERVE_GFX950_H

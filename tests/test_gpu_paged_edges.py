@@ -1,0 +1,112 @@
+"""The paged cache at its edges: bounds and lengths that cannot be, between
+guarded buffers.  Bars as in test_gpu_paged.py.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from conftest import rel_l2
+from oracle import paged_oracle as oracle
+from test_gpu_paged import TOL, Cache, dev  # noqa: F401  (dev is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+GUARD = 4096  # elements on either side
+
+
+class Guarded:
+    """A device tensor between two stretches of a pattern."""
+
+    def __init__(self, shape, dtype, dev, value=None):
+        n = 1
+        for d in shape:
+            n *= d
+        self.whole = torch.full((n + 2 * GUARD,), 77.0, dtype=dtype, device=dev)
+        self.t = self.whole[GUARD:GUARD + n].view(shape)
+        if value is not None:
+            self.t.copy_(value)
+
+    def intact(self):
+        return bool((self.whole[:GUARD] == 77).all() and (self.whole[-GUARD:] == 77).all())
+
+
+def guarded_step(c, dev, lens, cu):
+    """Append and attention through the C ABI, every buffer they write guarded;
+    returns (q, k_pages, v_pages, o, lse)."""
+    from delta_feedback_experiment_amd import _lib
+
+    N, Hq, D = c.q.shape
+    P, page, Hkv, _ = c.k_pages.shape
+    table, q, k, v = (t.to(dev) for t in (c.table, c.q, c.k, c.v))
+    kp, vp = (Guarded(t.shape, c.dtype, dev, t) for t in (c.k_pages, c.v_pages))
+    q_out, o = (Guarded(q.shape, c.dtype, dev) for _ in range(2))
+    lse = Guarded((N, Hq), torch.float32, dev)
+    at = lambda t: t.data_ptr()  # noqa: E731
+    common = dict(dtype=_lib.PKDA_BF16 if c.dtype == torch.bfloat16 else _lib.PKDA_F32, num_seqs=len(lens),
+                  num_tokens=N, q_heads=Hq, kv_heads=Hkv, head_dim=D, page_size=page, max_pages=table.shape[1],
+                  num_pages=P, table_stride=table.stride(0), cu_seqlens=at(cu), seq_lens=at(lens), page_table=at(table),
+                  k_pages=at(kp.t), v_pages=at(vp.t), k_page_stride=kp.t.stride(0), v_page_stride=vp.t.stride(0),
+                  q_stride=q.stride(0))
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.call("pkda_paged_append", _lib.PagedAppendArgs(q=at(q), k=at(k), v=at(v), k_stride=k.stride(0),
+                                                        v_stride=v.stride(0), q_out=at(q_out.t), **common), stream)
+    args = _lib.PagedAttentionArgs(q=at(q_out.t), scale=D ** -0.5, o=at(o.t), lse=at(lse.t), **common)
+    args.struct_size = ctypes.sizeof(args)
+    floats = _lib.lib().pkda_paged_attention_workspace(ctypes.byref(args))
+    work = Guarded((max(floats, 4),), torch.float32, dev)
+    args.workspace = at(work.t)
+    _lib.call("pkda_paged_attention", args, stream)
+    torch.cuda.synchronize()
+    assert all(x.intact() for x in (kp, vp, q_out, o, lse, work))
+    return q_out.t.cpu(), kp.t.cpu(), vp.t.cpu(), o.t.cpu(), lse.t.cpu()
+
+
+def untouched(c, kp, vp):
+    """Pages that no sequence owns are as they were."""
+    used = torch.zeros(c.pages, dtype=torch.bool)
+    used[c.table[(c.table >= 0) & (c.table < c.pages)].long()] = True
+    return torch.equal(kp[~used], c.k_pages[~used]) and torch.equal(vp[~used], c.v_pages[~used])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_clamped_bounds_and_lengths(dev, dtype):  # noqa: F811
+    """Bounds that rise once they are clamped to the packed length (the first one
+    counts as 0), and lengths clamped to the table's row, give the clamped ones' result."""
+    print(f"[gpu] paged cache, clamped bounds {dtype}", flush=True)
+    c = Cache([20, 30, 9], [4, 5, 6], 4, 2, 64, 8, dtype, seed=10, garbage=0.0, tail_pages=0)
+    room = c.table.shape[1] * 8
+    c.table[0], c.table[1], c.table[2] = torch.tensor([1, 0, 3, 2]), torch.tensor([7, 5, 4, 6]), -1
+    for cu in ([0, 4, 9, 900], [3, 4, 9, 15], [-5, -4, 2 ** 31 - 1, 15], [0, 4, 9, 11]):
+        for lens in ([20, 30, 9], [2 ** 31 - 1, -3, 9]):
+            got = guarded_step(c, dev, *(torch.tensor(x, dtype=torch.int32, device=dev) for x in (lens, cu)))
+            inside = torch.tensor([0, *(min(max(x, 0), 15) for x in cu[1:])])
+            short = torch.tensor([min(max(x, 0), room) for x in lens])
+            rq, rk, rv = oracle.append_reference(c.k, c.v, c.k_pages, c.v_pages, c.table, short, inside, c.q)
+            assert all(torch.equal(a.double(), b) for a, b in zip(got[:3], (rq, rk, rv))), (cu, lens)
+            assert untouched(c, got[1], got[2])
+            ro, rl = oracle.attention_reference(rq.to(dtype), got[1], got[2], c.table, short, inside)
+            assert rel_l2(got[3].float(), ro) < TOL[dtype], (cu, lens)
+            assert torch.equal(torch.isneginf(got[4]), torch.isneginf(rl))
+
+
+@pytest.mark.parametrize("S,N,Hq,Hkv", [(3, 60, 64, 4), (70, 300, 64, 4), (70, 300, 64, 64), (200, 3000, 16, 2),
+                                        (5, 3000, 64, 16)])
+def test_falling_bounds_stay_inside(dev, S, N, Hq, Hkv):  # noqa: F811
+    """Bounds that fall name no sequences: nothing past a buffer is read or
+    written, nothing in a page that no sequence has."""
+    print(f"[gpu] paged cache, falling bounds {S} sequences {N} tokens", flush=True)
+    gen = torch.Generator().manual_seed(S + N)
+    new = [N // S] * S
+    c = Cache([n + 5 for n in new], new, Hq, Hkv, 32, 8, torch.bfloat16, seed=31, garbage=0.0, tail=N - sum(new))
+    lens = c.lens.to(dev)
+    for _ in range(4):
+        cu = torch.randint(-5, N + 5, (S + 1,), generator=gen, dtype=torch.int32).to(dev)
+        _, kp, vp, _, _ = guarded_step(c, dev, lens, cu)
+        assert untouched(c, kp, vp)
+    falls = torch.arange(S, -1, -1, dtype=torch.int32).mul(N // S).to(dev)
+    _, kp, vp, _, _ = guarded_step(c, dev, lens, falls)
+    assert untouched(c, kp, vp)
