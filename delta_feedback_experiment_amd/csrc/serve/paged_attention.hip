@@ -811,7 +811,7 @@ __device__ __forceinline__ void attend_rows(const AttnParams& p, unsigned block,
       run.step(s, p.scale2, tile.rows > kRowTile / 2 ? kSlack : 0.f);
 #pragma unroll
       for (int n = 0; n < 2; ++n) mma_values<T, D>(run.o, sk + kTileBytes, 32 * n, s[n], lane);
-      const uint64_t bad = __builtin_amdgcn_readfirstlane(odd.x) |
+      const uint64_t bad = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(odd.x) |
                            (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(odd.y) << 32;
       if (bad) add_nonfinite<T, D, 2>(run.o, s, bad, p, tile.n, kvh, key0, row.pos, lane);
     }

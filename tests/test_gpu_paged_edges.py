@@ -1,10 +1,12 @@
 """The paged cache at its edges: bounds and lengths that cannot be, between
-guarded buffers.  Bars as in test_gpu_paged.py.
+guarded buffers, and tables without an entry to spare.  Bars as in
+test_gpu_paged.py.
 """
 
 from __future__ import annotations
 
 import ctypes
+import math
 
 import pytest
 import torch
@@ -110,3 +112,29 @@ def test_falling_bounds_stay_inside(dev, S, N, Hq, Hkv):  # noqa: F811
     falls = torch.arange(S, -1, -1, dtype=torch.int32).mul(N // S).to(dev)
     _, kp, vp, _, _ = guarded_step(c, dev, lens, falls)
     assert untouched(c, kp, vp)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("page", [1, 5, 16])
+def test_a_bad_value_at_the_middle_of_the_last_tile(dev, dtype, page):  # noqa: F811
+    """The last position is key 31 of a tile of 64, its value is not finite and
+    the table ends there: the keys after it, which do not exist, are not looked
+    up (the table is a view, with entries of the pool's behind each row)."""
+    from delta_feedback_experiment_amd import paged_attention
+
+    print(f"[gpu] paged attention, bad value at key 31 {dtype} pages of {page}", flush=True)
+    c = Cache([160, 160], [100, 100], 128, 128, 32, page, dtype, seed=34, tail_pages=0, garbage=0.0)
+    assert c.table.shape[1] * page == 160
+    wide = torch.zeros(2, c.table.shape[1] + 64, dtype=torch.int32, device=dev)
+    wide[:, :c.table.shape[1]] = c.table.to(dev)
+    table, lens, cu = wide[:, :c.table.shape[1]], c.lens.to(dev), c.cu.to(dev)
+
+    def attend():
+        return paged_attention(c.q.to(dev), c.k_pages.to(dev), c.v_pages.to(dev), table, lens, cu_seqlens=cu)
+
+    clean, lse0 = attend()
+    c.v_pages[int(c.table[1, 159 // page]), 159 % page, :, 5] = math.nan
+    o, lse = attend()
+    assert torch.equal(lse, lse0) and torch.isnan(o[199, :, 5]).all()
+    o[199, :, 5] = clean[199, :, 5]
+    assert torch.equal(o, clean)
