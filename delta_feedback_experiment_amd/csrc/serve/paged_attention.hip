@@ -928,9 +928,8 @@ struct Plan {
 // Which form takes which sequences, and into how many splits a sequence's keys
 // are cut at most, from what the host knows: sequences have num_tokens /
 // num_seqs tokens each.  Times are BF16, heads of 128, unless they say more.
-Plan plan(AttnParams& p) {
+Plan plan(AttnParams& p, bool packed) {
   const int64_t group = p.group.d, N = p.s.num_tokens, S = p.s.num_seqs, heads = p.kv_heads;
-  const bool packed = p.s.cu != nullptr;
   Plan r;
   // More than 32 rows a sequence go to 128-row tiles: 13 prompts take 84 us so,
   // and 238 as tiles of 32 rows; 64 sequences of 40 rows after 1,900 keys 81 and
@@ -970,7 +969,7 @@ Plan plan(AttnParams& p) {
 
 template <typename T, int D>
 int launch_attention(AttnParams p, hipStream_t s) {
-  const Plan r = plan(p);
+  const Plan r = plan(p, p.s.cu != nullptr);
   const int64_t per_tile = (int64_t)p.kv_heads * p.splits;
   const int64_t blocks = (r.row_tiles + r.key_tiles) * per_tile;
   const int64_t rows = (int64_t)p.s.num_tokens * p.q_heads;
@@ -1014,7 +1013,7 @@ int attention_sizes(const pkda_paged_attention_args* a, AttnParams& p) {
   p.group = FastDiv::make((uint32_t)(a->q_heads / a->kv_heads));
   PKDA_REQUIRE((int64_t)a->num_tokens * p.group.d <= 1 << 30, PKDA_EINVAL, "%d tokens of %d heads", a->num_tokens,
                a->q_heads);
-  plan(p);
+  plan(p, p.s.cu != nullptr);
   return 0;
 }
 
@@ -1024,7 +1023,14 @@ int attention_sizes(const pkda_paged_attention_args* a, AttnParams& p) {
 extern "C" int64_t pkda_paged_attention_workspace(const pkda_paged_attention_args* a) {
   pkda::AttnParams p;
   if (pkda::attention_sizes(a, p)) return -1;
-  return p.splits > 1 ? (int64_t)p.splits * a->num_tokens * a->q_heads * (a->head_dim + 2) : 0;
+  // by the sizes alone: one token a sequence may come with cu_seqlens or without
+  pkda::plan(p, true);
+  int splits = p.splits;
+  if (a->num_tokens == a->num_seqs) {
+    pkda::plan(p, false);
+    splits = splits > p.splits ? splits : p.splits;
+  }
+  return splits > 1 ? (int64_t)splits * a->num_tokens * a->q_heads * (a->head_dim + 2) : 0;
 }
 
 extern "C" int pkda_paged_attention(const pkda_paged_attention_args* a, void* stream) {

@@ -111,8 +111,9 @@ typedef struct pkda_paged_attention_args {
   float* workspace;             /* pkda_paged_attention_workspace() floats */
 } pkda_paged_attention_args;
 
-/* Floats of workspace the call needs, from its sizes alone (no pointer is
- * read); < 0 for sizes the call refuses. */
+/* Floats of workspace the call needs at most, from its sizes alone (no pointer
+ * is looked at, cu_seqlens neither: where num_tokens == num_seqs it is enough
+ * with cu_seqlens and without); < 0 for sizes the call refuses. */
 int64_t pkda_paged_attention_workspace(const pkda_paged_attention_args* args);
 int pkda_paged_attention(const pkda_paged_attention_args* args, void* stream);
 

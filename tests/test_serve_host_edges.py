@@ -2,7 +2,10 @@
 
 from __future__ import annotations
 
+import ctypes
 import re
+
+import pytest
 
 from conftest import ROOT
 
@@ -21,3 +24,23 @@ def test_lane_reads_are_widened_without_their_sign():
                 found += 1
                 assert statement[:m.start()].endswith("(uint32_t)"), (path.name, statement.strip())
     assert found
+
+
+@pytest.mark.parametrize("tokens,seqs,heads,kv_heads,positions", [
+    (200, 1, 4, 1, 1024), (300, 1, 8, 2, 2048), (1, 1, 32, 8, 131072), (64, 64, 32, 8, 4096), (5, 5, 64, 64, 4096),
+    (320, 64, 32, 4, 4096), (2048, 1, 32, 8, 16384), (500, 500, 96, 32, 65536), (300, 300, 96, 3, 4096)])
+def test_workspace_follows_from_the_sizes(tokens, seqs, heads, kv_heads, positions):
+    """The same length whether cu_seqlens is there yet or not, and enough for
+    the form that takes more."""
+    from delta_feedback_experiment_amd import _lib
+
+    handle = _lib.lib()
+
+    def floats(**kw):
+        args = _lib.PagedAttentionArgs(dtype=1, num_seqs=seqs, num_tokens=tokens, q_heads=heads, kv_heads=kv_heads,
+                                       head_dim=128, page_size=64, max_pages=positions // 64, num_pages=9, **kw)
+        args.struct_size = ctypes.sizeof(args)
+        return handle.pkda_paged_attention_workspace(ctypes.byref(args))
+
+    assert floats() == floats(cu_seqlens=16) >= 0
+    assert floats() % (tokens * heads * 130) == 0  # so many rows' sums and outputs a split
