@@ -770,9 +770,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
       }
       const float base = mine == -INFINITY ? 0.f : mine;
       float part = 0.f;
-      if (fabsf(base) < 0x1p40f) {
+      if (fabsf(base) < 0x1p20f) {
         // l log2 e - base log2 e in one operation, and the rounding of the second
-        // product, which is common to all, afterwards
+        // product, which is common to all, afterwards (up to 1/16 here; past 2^31 it
+        // would leave the range of the exponential, and 0 times infinity)
         const float product = base * kLog2e;
 #pragma unroll
         for (int u = 0; u < 4; ++u)

@@ -1,0 +1,30 @@
+"""Sampling on the GPU at its edges, against the 64-bit oracle: bars as in test_gpu_sample.py."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_sample import SETTINGS, check, dev, gumbel  # noqa: F401  (dev is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("large", [1e6, 1e9, 6e9, 1e10, 1e11, 1e12, 3e12, 1e30])
+def test_large_finite_logits(dev, dtype, large):  # noqa: F811
+    """Most of a row, and whole waves of it, masked with a large negative number;
+    and rows whose every logit is large, of either sign."""
+    print(f"[gpu] sample, logits of {large:g} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(17)
+    n, V = len(SETTINGS), 40011
+    noise = gumbel(n, V, seed=18)
+    logits = torch.full((n, V), -large)
+    logits[:, 30000:30300] = 3 * torch.randn(n, 300, generator=gen)
+    logits[:, V - 1] = 0.5
+    check(dev, logits.to(dtype), noise, SETTINGS)
+    for sign in (-1, 1):
+        logits = sign * large * (1 + torch.randint(0, 3, (n, 9001), generator=gen) * 2.0 ** -6)
+        check(dev, logits.to(dtype), noise[:, :9001].contiguous(), SETTINGS)
