@@ -902,13 +902,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
           if (t > best && x >= least)
             if (float_key(x) > edge || order_key(x, i) >= low)
               if (min_p <= 0.f || expf(s.z(x)) >= min_p) {
-                best = fminf(t, kMaxFloat);
+                best = t;
                 at = i;
               }
         };
         if (s.inv != 0.f) row.each_with_noise([&](float x, float g, int i) { dense(x, s.z_fast(x), g, i); });
         else row.each_with_noise([&](float x, float g, int i) { dense(x, s.z(x), g, i); });
-        if (best > -INFINITY) pick = ((uint64_t)float_key(best) << 32) | (uint32_t)~at;
+        if (best > -INFINITY) pick = ((uint64_t)float_key(fminf(best, kMaxFloat)) << 32) | (uint32_t)~at;
       }
     }
     pick = block_reduce(pick, lds.wave_k, max_key);

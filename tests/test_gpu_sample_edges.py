@@ -28,3 +28,16 @@ def test_large_finite_logits(dev, dtype, large):  # noqa: F811
     for sign in (-1, 1):
         logits = sign * large * (1 + torch.randint(0, 3, (n, 9001), generator=gen) * 2.0 ** -6)
         check(dev, logits.to(dtype), noise[:, :9001].contiguous(), SETTINGS)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [5003, 50304])
+def test_infinite_noise_ties_at_the_lowest_index(dev, dtype, vocab):  # noqa: F811
+    """Noise of +inf at two tokens: of one load, of one thread, of two threads."""
+    print(f"[gpu] sample, infinite noise {dtype} {vocab}", flush=True)
+    gen = torch.Generator().manual_seed(19)
+    logits = torch.randn(len(SETTINGS), vocab, generator=gen).to(dtype)
+    for pair in ([8, 9], [8, 11], [8, 8 + 4096], [700, 9]):
+        noise = gumbel(len(SETTINGS), vocab, seed=20)
+        noise[:, pair] = math.inf
+        check(dev, logits, noise, SETTINGS)
