@@ -463,7 +463,9 @@ struct Scale {
   __device__ __forceinline__ void init(float top, float t) {
     m = top;
     temperature = t;
-    c = fminf(kLog2e / t, kMaxFloat);
+    // above 0 also for an infinite temperature: -inf has the weight 0, not NaN, and
+    // a finite logit one within 2^-21 of 1
+    c = fmaxf(fminf(kLog2e / t, kMaxFloat), 0x1p-149f);
     // l c - m c in one operation: every weight of a row is off by one factor, the
     // rounding of m c, which must stay near 1
     const bool near = fabsf(m * c) <= 0x1p20f;
@@ -482,7 +484,8 @@ struct Scale {
     q = __builtin_fmaf(__builtin_fmaf(-q, temperature, d), inv, q);
     return __builtin_fmaf(__builtin_fmaf(-q, temperature, d), inv, q);
   }
-  __device__ __forceinline__ float z(float x) const { return (x - m) / temperature; }
+  // (the difference of two finite logits is finite)
+  __device__ __forceinline__ float z(float x) const { return fmaxf(x - m, -kMaxFloat) / temperature; }
 };
 
 // How a round divides an interval of keys: rows 1 .. n, falling, exactly; row 0 is
@@ -567,7 +570,7 @@ __device__ __forceinline__ Ending find_ending(const RowData<T>& row, const Scale
   // the first round goes from the top in steps of half an e-fold, the rest in the
   // last row; a later one divides its interval, or (open) goes on from its top in
   // steps of all the bins before
-  float width = mass ? 0.5f * s.temperature : 0.5f;
+  float width = mass ? fminf(0.5f * s.temperature, kMaxFloat) : 0.5f;
   bool open = true;
   for (int round = 0;; ++round) {
     Bins b;

@@ -44,8 +44,8 @@ def sample_tokens(
 
     The token is the lowest index that maximises ``z + noise`` over what is
     left: a draw from the softmax over it.  ``temperature <= 0`` takes the
-    first token.  ``token [rows]`` int32; ``logprob [rows]`` FP32 is its
-    ``log_softmax(logits)``, before any setting.
+    first token, an infinite one makes every ``z`` 0.  ``token [rows]`` int32;
+    ``logprob [rows]`` FP32 is its ``log_softmax(logits)``, before any setting.
 
     Logits of NaN or -inf are never taken, +inf counts as the largest finite
     number; a row that holds nothing else gives token -1 and logprob -inf.

@@ -41,3 +41,19 @@ def test_infinite_noise_ties_at_the_lowest_index(dev, dtype, vocab):  # noqa: F8
         noise = gumbel(len(SETTINGS), vocab, seed=20)
         noise[:, pair] = math.inf
         check(dev, logits, noise, SETTINGS)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [math.inf, 3e38, 1e30])
+@pytest.mark.parametrize("vocab", [4099, 50303])
+def test_temperatures_without_bound(dev, dtype, temperature, vocab):  # noqa: F811
+    """z is 0, or nearly, for every finite logit: a uniform draw over what the
+    settings leave.  Rows with -inf, with the type's lowest value, and without."""
+    print(f"[gpu] sample, temperature {temperature:g} {dtype} {vocab}", flush=True)
+    gen = torch.Generator().manual_seed(21)
+    settings = [{**s, "temperature": temperature} for s in SETTINGS]
+    for other in (None, -math.inf, float(torch.finfo(dtype).min)):
+        logits = 3 * torch.randn(len(settings), vocab, generator=gen)
+        if other is not None:
+            logits[:, 1::2] = other
+        check(dev, logits.to(dtype), gumbel(*logits.shape, seed=22), settings)
