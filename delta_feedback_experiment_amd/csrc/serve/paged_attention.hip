@@ -6,8 +6,7 @@
 // any number.  Scores, softmax and output run in one pass over the keys with
 // the row's running maximum m and sum l (base 2, FP32):
 //   m' = max(m, max_s S),  p = 2^(S - m'),  l = l 2^(m - m') + sum_s p,
-//   O = O 2^(m - m') + p V,   o = O / l,  lse = (m + log2 l) ln 2,
-// which hold for any m; it stays near the maximum (kSlack below).
+//   O = O 2^(m - m') + p V,   o = O / l,  lse = (m + log2 l) ln 2.
 //
 // Products.  Both are taken transposed, S^T = K Q^T and O^T = V^T P^T, as
 // 32x32 MFMA tiles.  A lane then holds one query row (its column) and 16 of a
@@ -34,12 +33,12 @@
 // What bounds it, measured in BF16 with heads of 128 (a large read runs at 4.0 to
 // 5.0 TB/s, a large matrix product at 1188 TFLOP/s).  Decode, 256 sequences of
 // 2,600 keys, 32/8 heads: 546 us, 4.98 TB/s of keys and values.  One sequence of
-// 131,072 keys: 114 us, 4.7 TB/s.  2,048 tokens after 14,336, 32/8 heads: 585 us,
-// 880 TFLOP/s: a wave's 32 products a tile are 1,024 cycles, its 246 vector
+// 131,072 keys: 114 us, 4.7 TB/s.  2,048 tokens after 14,336, 32/8 heads: 603 us,
+// 855 TFLOP/s: a wave's 32 products a tile are 1,024 cycles, its 246 vector
 // instructions, 32 exponentials among them, about 1,370, and its reads of LDS
 // about 800; the other workgroup's wave on the SIMD overlaps them only in part
-// (2,400 cycles a tile and wave).  13 prompts of 250 to 1,659 tokens, 16/4 heads:
-// 84 us, 606 TFLOP/s: 6 us of a row tile's 33 are its way to its first keys and
+// (2,500 cycles a tile and wave).  13 prompts of 250 to 1,659 tokens, 16/4 heads:
+// 87 us, 588 TFLOP/s: 6 us of a row tile's 33 are its way to its first keys and
 // its output.
 #include <math.h>
 
@@ -266,7 +265,7 @@ __device__ __forceinline__ int wave_sum(int x) {
 // a sequence has one tile a level from lo up, so the tiles from a level up are
 // counted by one sum over the wave, and the level of the t-th by bisection.  In
 // the sequences' order instead the last long ones begin when the rest is nearly
-// done: 13 prompts of 250 to 1,659 tokens 99 us, so 84.
+// done: 13 prompts of 250 to 1,659 tokens 106 us, so 87.
 template <int M>
 __device__ __forceinline__ bool find_longest(const AttnParams& p, int t, Tile& tile) {
   const int lane = threadIdx.x & 63;
@@ -335,17 +334,15 @@ __device__ __forceinline__ void arrived(u32x4 (&q)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(q[i]));
 }
 
-// A row's softmax while its keys pass.  m is a maximum of the keys so far, or less
-// by up to `slack` (probabilities are then at most 2^slack).  With the exact one
-// some row of a wave raises it, and all of a tile's outputs are rescaled, in nearly
-// every tile of the first fifty: 2,048 tokens after 14,336 599 us, and 585 with a
-// slack of 8; 13 prompts 87 and 84.  But the largest probability is then no longer
-// 1, which BF16 holds exactly: the output's error against 64 bits is 0.0023 of its
-// size, and 0.0020 with the exact maximum (0.0017 is the output's own rounding).
-// Few rows (up to half a tile of 128), which wait for memory, keep the exact one.
-constexpr float kSlack = 8.f;
+// A row's softmax while its keys pass.  m is their exact maximum, so the likeliest
+// key's probability is 1, which BF16 holds.  Some row of a wave raises it, and all
+// of a tile's outputs are rescaled, in nearly every tile of the first fifty:
+// followed only where it has grown by more than 2^8, 2,048 tokens after 14,336 take
+// 584 us and not 603, 13 prompts 84 and not 87, but that probability is then rounded
+// with the others: the output's error against 64 bits is 0.0023 of its size, so
+// 0.0020 (0.0017 is the output's own rounding).
 template <int DT> struct Running {
-  float m, l;  // m (base 2), and the sum over this half's keys
+  float m, l;  // maximum (base 2), and the sum over this half's keys
   f32x16 o[DT];
   __device__ __forceinline__ void init() {
     m = -INFINITY;
@@ -357,16 +354,15 @@ template <int DT> struct Running {
   }
   // scores of N tiles of keys -> their probabilities
   template <int N>
-  __device__ __forceinline__ void step(f32x16 (&s)[N], float scale2, float slack) {
+  __device__ __forceinline__ void step(f32x16 (&s)[N], float scale2) {
     float mx = s[0][0];
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     mx = join_halves(mx, [](float a, float b) { return fmaxf(a, b); }) * scale2;
-    const bool grown = mx > m + slack;
-    if (__any(grown)) {
-      const float mn = grown ? mx : m;
+    if (__any(mx > m)) {
+      const float mn = fmaxf(m, mx);
       const float a = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
       m = mn;
       l *= a;
@@ -569,7 +565,7 @@ __device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block,
         if (key0 + i > row.pos || !((there >> i) & 1)) s[0][r] = -INFINITY;
       }
     }
-    run.step(s, p.scale2, 0.f);
+    run.step(s, p.scale2);
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     mma_values<T, D>(run.o, sv, 0, s[0], lane);
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
@@ -636,7 +632,7 @@ constexpr int kKeyTile = 64;
 // WHOLE: the rows that a wave stages at a time, 64 / NC keys, lie in one page
 // (the page size is a multiple of them): a load's address is the page's, in
 // scalar registers, and a lane's constant part.  2,048 tokens after 14,336:
-// 585 us, with every lane's own addresses 626; 13 prompts: 84 and 88.
+// 603 us, with every lane's own addresses 645; 13 prompts: 87 and 91.
 template <typename T, int D> struct RowsLds {
   __align__(16) char kv[4 * kKeyTile * Geo<T, D>::RB];  // two stages of K, V
   // of tile t % 3: its keys with values that are not finite, and those without a page
@@ -808,7 +804,7 @@ __device__ __forceinline__ void attend_rows(const AttnParams& p, unsigned block,
           for (int r = 0; r < 16; ++r)
             if (((n ? gone1 : gone0) >> key_of(r, half)) & 1) s[n][r] = -INFINITY;
       }
-      run.step(s, p.scale2, tile.rows > kRowTile / 2 ? kSlack : 0.f);
+      run.step(s, p.scale2);
 #pragma unroll
       for (int n = 0; n < 2; ++n) mma_values<T, D>(run.o, sk + kTileBytes, 32 * n, s[n], lane);
       const uint64_t bad = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(odd.x) |
@@ -931,7 +927,7 @@ struct Plan {
 Plan plan(AttnParams& p, bool packed) {
   const int64_t group = p.group.d, N = p.s.num_tokens, S = p.s.num_seqs, heads = p.kv_heads;
   Plan r;
-  // More than 32 rows a sequence go to 128-row tiles: 13 prompts take 84 us so,
+  // More than 32 rows a sequence go to 128-row tiles: 13 prompts take 87 us so,
   // and 238 as tiles of 32 rows; 64 sequences of 40 rows after 1,900 keys 81 and
   // 101.  Not where those tiles leave the card half empty: one prompt of 1,531
   // tokens, 8/2 heads, is 98 of them (47 us) or 386 of 32 rows (36 us).

@@ -138,3 +138,26 @@ def test_a_bad_value_at_the_middle_of_the_last_tile(dev, dtype, page):  # noqa: 
     assert torch.equal(lse, lse0) and torch.isnan(o[199, :, 5]).all()
     o[199, :, 5] = clean[199, :, 5]
     assert torch.equal(o, clean)
+
+
+@pytest.mark.parametrize("lens,new,Hq,Hkv", [([300, 65], [150, 65], 64, 64), ([300], [1], 8, 2),
+                                             ([300, 9], [40, 9], 4, 2)])
+def test_the_likeliest_key_is_not_rounded(dev, lens, new, Hq, Hkv):  # noqa: F811
+    """One key of the second tile has a larger score than the others, by less
+    than 2^8 for most rows, and the only value: its probability against the row's
+    maximum is 1, so the output is rounded once (FP32 sums: 1e-5 before that)."""
+    print(f"[gpu] paged attention, likeliest key {lens} {Hq}/{Hkv}", flush=True)
+    c = Cache(lens, new, Hq, Hkv, 64, 16, torch.bfloat16, seed=33, garbage=0.0)
+    kept = c.v_pages.clone()
+    c.k_pages.zero_()
+    c.v_pages.zero_()
+    for n, length in enumerate(lens):
+        at = 70 if length > 70 else 3
+        where = int(c.table[n, at // 16]), at % 16
+        c.k_pages[where][:, 0] = 1.0
+        c.v_pages[where] = kept[where]
+    c.q.abs_()
+    o, _ = c.attend(dev, scale=1.0)
+    ro, _ = oracle.attention_of_sequences(c.q, c.k_pages, c.v_pages, c.table, c.lens, c.cu, 1.0)
+    slack = 1e-5 * ro.abs()
+    assert ((o.cpu() >= (ro - slack).bfloat16()) & (o.cpu() <= (ro + slack).bfloat16())).all()
