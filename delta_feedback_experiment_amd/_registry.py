@@ -140,16 +140,18 @@ def call(op, *args):
 
 def launch(op, *args):
     """The device kernel of ``op`` itself, where the dispatcher has nothing to
-    add to it: plain tensors, which the caller has found on one HIP device,
-    nothing that asks for gradients, and no mode, transform, trace or profiler
-    that would see the operator; elsewhere :func:`call`.  The way through the
-    dispatcher and back into Python is 4 us of a call that takes 16 in all."""
-    if (torch.compiler.is_compiling() or _C._len_torch_dispatch_stack() or _C._get_tracing_state() is not None
+    add to it: plain tensors, which the caller has found on one device, that of
+    HIP and not the meta one, none a lazy negation; nothing that asks for
+    gradients; no mode, transform, trace or profiler that would see the
+    operator.  Elsewhere :func:`call`: the way through the dispatcher and back
+    into Python is 4 us of a call."""
+    if (torch.compiler.is_compiling() or not args[0].is_cuda or _C._len_torch_dispatch_stack()
+            or _C._len_torch_function_stack() or _C._get_tracing_state() is not None
             or _C._functorch.peek_interpreter_stack() is not None or _C._autograd._profiler_enabled()
             or (_C.is_grad_enabled() and _C._any_requires_grad(*args))):
         return call(op, *args)
     for t in args:
-        if isinstance(t, Tensor) and type(t) not in _PLAIN:
+        if isinstance(t, Tensor) and (type(t) not in _PLAIN or t.is_neg()):
             return call(op, *args)
     if _WRITTEN[op]:
         _raise_versions(op, args)

@@ -161,3 +161,38 @@ def test_the_likeliest_key_is_not_rounded(dev, lens, new, Hq, Hkv):  # noqa: F81
     ro, _ = oracle.attention_of_sequences(c.q, c.k_pages, c.v_pages, c.table, c.lens, c.cu, 1.0)
     slack = 1e-5 * ro.abs()
     assert ((o.cpu() >= (ro - slack).bfloat16()) & (o.cpu() <= (ro + slack).bfloat16())).all()
+
+
+def test_function_modes_and_lazy_negations(dev):  # noqa: F811
+    """A function mode sees the operators, and a lazily negated view is negated."""
+    from torch.overrides import TorchFunctionMode
+
+    from delta_feedback_experiment_amd import paged_append_, paged_attention, sample_tokens
+
+    print("[gpu] paged cache, function modes", flush=True)
+    c = Cache([3, 9], [1, 1], 4, 2, 64, 8, torch.float32, seed=35, cu=False, garbage=0.0)
+    table, lens, _ = c.tables(dev)
+    q, k, v = (t.to(dev) for t in (c.q, c.k, c.v))
+    logits, noise = torch.randn(2, 100, device=dev), torch.randn(2, 100, device=dev)
+
+    def run(q, k, logits):
+        kp, vp = c.k_pages.to(dev), c.v_pages.to(dev)
+        out = paged_append_(k, v, kp, vp, table, lens, q=q)
+        return (out, kp, vp, *paged_attention(q, kp, vp, table, lens), *sample_tokens(logits, noise))
+
+    class Watch(TorchFunctionMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = set()
+
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            self.seen.add(str(func))
+            return func(*args, **(kwargs or {}))
+
+    with Watch() as watch:
+        watched = run(q, k, logits)
+    for name in ("paged_append_", "paged_attention", "sample_tokens"):
+        assert any(name in f for f in watch.seen), name
+    assert all(torch.equal(a, b) for a, b in zip(watched, run(q, k, logits)))
+    negated = run(*(torch._neg_view(t) for t in (q, k, logits)))
+    assert all(torch.equal(a, b) for a, b in zip(negated, run(-q, -k, -logits)))

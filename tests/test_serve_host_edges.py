@@ -6,6 +6,7 @@ import ctypes
 import re
 
 import pytest
+import torch
 
 from conftest import ROOT
 
@@ -44,3 +45,29 @@ def test_workspace_follows_from_the_sizes(tokens, seqs, heads, kv_heads, positio
 
     assert floats() == floats(cu_seqlens=16) >= 0
     assert floats() % (tokens * heads * 130) == 0  # so many rows' sums and outputs a split
+
+
+def _meta_case():
+    def z(*shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    i32 = dict(dtype=torch.int32)
+    return z(4, 4, 64), z(4, 2, 64), z(3, 16, 2, 64), z(2, 3, **i32), z(2, **i32), z(3, **i32), z(48, 32)
+
+
+def test_meta_tensors_get_their_shapes():
+    """On the meta device, as the operators themselves and the decode step take it."""
+    from delta_feedback_experiment_amd import paged_append_, paged_attention, sample_tokens
+
+    q, kv, pages, table, lens, cu, angle = _meta_case()
+    out = paged_append_(kv, kv, pages, pages, table, lens, cu_seqlens=cu, q=q, cos=angle, sin=angle)
+    assert out.is_meta and out.shape == q.shape and out.dtype == q.dtype
+    assert paged_append_(kv, kv, pages, pages, table, lens, cu_seqlens=cu) is None
+    o, lse = paged_attention(q, pages, pages, table, lens, cu_seqlens=cu)
+    assert o.is_meta and o.shape == q.shape and lse.shape == (4, 4) and lse.dtype == torch.float32
+    logits = torch.empty(3, 10, dtype=torch.bfloat16, device="meta")
+    token, logprob = sample_tokens(logits, logits.float(), top_k=5)
+    assert token.is_meta and token.shape == logprob.shape == (3,)
+    assert token.dtype == torch.int32 and logprob.dtype == torch.float32
+    with pytest.raises(ValueError, match="share"):
+        paged_attention(q[:, :3], pages, pages, table, lens, cu_seqlens=cu)
