@@ -81,7 +81,8 @@ def _check_cache(name: str, x: Tensor, k_pages: Tensor, v_pages: Tensor, page_ta
         raise ValueError(f"cu_seqlens must be int32 [{S + 1}]")
     for t in (k_pages, v_pages):
         stride = t.stride()
-        if (stride[3] != 1 or stride[2] != D or stride[1] != H * D or not _aligned(t, stride[0])) and t.numel():
+        if (stride[3] != 1 or (stride[2] != D and H > 1) or (stride[1] != H * D and R > 1)
+                or not _aligned(t, stride[0])) and t.numel():
             raise ValueError("every page must be dense, in whole 16 bytes")
 
 

@@ -196,3 +196,21 @@ def test_function_modes_and_lazy_negations(dev):  # noqa: F811
     assert all(torch.equal(a, b) for a, b in zip(watched, run(q, k, logits)))
     negated = run(*(torch._neg_view(t) for t in (q, k, logits)))
     assert all(torch.equal(a, b) for a, b in zip(negated, run(-q, -k, -logits)))
+
+
+def test_pages_of_one_head_kept_by_head(dev):  # noqa: F811
+    """Pools [pages, 1, page_size, head_dim], turned: dense all the same."""
+    from delta_feedback_experiment_amd import paged_append_, paged_attention
+
+    print("[gpu] paged cache, one head", flush=True)
+    c = Cache([3, 30], [2, 30], 4, 1, 64, 8, torch.bfloat16, seed=36, garbage=0.0)
+    table, lens, cu = c.tables(dev)
+    q, k, v = (t.to(dev) for t in (c.q, c.k, c.v))
+    runs = []
+    for turned in (False, True):
+        kp, vp = (t.to(dev) for t in (c.k_pages, c.v_pages))
+        if turned:
+            kp, vp = (t.view(c.pages, 1, 8, 64).transpose(1, 2) for t in (kp, vp))
+        out = paged_append_(k, v, kp, vp, table, lens, cu_seqlens=cu, q=q)
+        runs.append((out, kp, vp, *paged_attention(out, kp, vp, table, lens, cu_seqlens=cu)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from conftest import ROOT
+from test_serve_host import _append, _attention, _case, _fake
 
 CSRC = ROOT / "delta_feedback_experiment_amd" / "csrc"
 
@@ -71,3 +72,16 @@ def test_meta_tensors_get_their_shapes():
     assert token.dtype == torch.int32 and logprob.dtype == torch.float32
     with pytest.raises(ValueError, match="share"):
         paged_attention(q[:, :3], pages, pages, table, lens, cu_seqlens=cu)
+
+
+@pytest.mark.parametrize("pages", [torch.zeros(3, 1, 16, 64).transpose(1, 2), torch.zeros(3, 64)[:, None, None],
+                                   torch.zeros(1, 3, 64).permute(1, 0, 2)[:, None]])
+def test_dense_pages_of_one_head_or_one_row(pages):
+    """The stride of an axis of length one says nothing."""
+    assert pages.is_contiguous() and pages.shape[2] == 1
+    page = pages.shape[1]
+    x, mode = _fake(_case(k=torch.zeros(4, 1, 64), v=torch.zeros(4, 1, 64), k_pages=pages, v_pages=pages,
+                          page_table=torch.zeros(2, 48 // page, dtype=torch.int32)))
+    with mode:
+        assert _append(x).shape == x["q"].shape
+        assert _attention(x)[0].shape == x["q"].shape
