@@ -939,7 +939,7 @@ Plan plan(AttnParams& p, bool packed) {
   // A row's part of a split costs 2 D floats, a key 2 D numbers a tile: enough
   // keys a split that the parts stay a small share.  8 keys a row of the tile:
   // the 64 sequences of 40 rows take 81 us, with 16 they take 83.
-  const int64_t per_seq = S > 0 ? (N * group + S - 1) / S : 1;
+  const int64_t per_seq = S > 0 && N > 0 ? (N * group + S - 1) / S : 1;
   const int64_t tile_rows = per_seq < 32 || p.key_rows != 32 ? (per_seq < 32 ? per_seq : 32)
                                                              : (per_seq < kRowTile ? per_seq : kRowTile);
   p.min_chunk = (int)((8 * tile_rows + kMinChunk - 1) / kMinChunk * kMinChunk);

@@ -214,3 +214,18 @@ def test_pages_of_one_head_kept_by_head(dev):  # noqa: F811
         out = paged_append_(k, v, kp, vp, table, lens, cu_seqlens=cu, q=q)
         runs.append((out, kp, vp, *paged_attention(out, kp, vp, table, lens, cu_seqlens=cu)))
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_a_step_without_tokens(dev):  # noqa: F811
+    """Live sequences, none of which has a new token."""
+    from delta_feedback_experiment_amd import paged_append_, paged_attention
+
+    print("[gpu] paged cache, no tokens", flush=True)
+    c = Cache([20, 3], [0, 0], 4, 2, 64, 8, torch.bfloat16, seed=37, garbage=0.0)
+    table, lens, cu = c.tables(dev)
+    q, k, v, kp, vp = (t.to(dev) for t in (c.q, c.k, c.v, c.k_pages, c.v_pages))
+    out = paged_append_(k, v, kp, vp, table, lens, cu_seqlens=cu, q=q)
+    o, lse = paged_attention(q, kp, vp, table, lens, cu_seqlens=cu)
+    torch.cuda.synchronize()
+    assert out.shape == o.shape == (0, 4, 64) and lse.shape == (0, 4)
+    assert torch.equal(kp.cpu(), c.k_pages) and torch.equal(vp.cpu(), c.v_pages)

@@ -4,6 +4,8 @@ from __future__ import annotations
 
 import ctypes
 import re
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -85,3 +87,23 @@ def test_dense_pages_of_one_head_or_one_row(pages):
     with mode:
         assert _append(x).shape == x["q"].shape
         assert _attention(x)[0].shape == x["q"].shape
+
+
+@pytest.mark.parametrize("seqs", [0, 1, 7])
+def test_no_tokens_of_some_sequences(seqs):
+    """Nothing to do is no error, and no division by the rows a sequence has; in
+    a process of its own, which a division by zero would end."""
+    code = f"""
+import ctypes
+from delta_feedback_experiment_amd import _lib
+common = dict(dtype=1, num_seqs={seqs}, num_tokens=0, q_heads=4, kv_heads=2, head_dim=64, page_size=16, max_pages=3,
+              num_pages=5, table_stride=3, cu_seqlens=16, seq_lens=16, page_table=16, k_pages=16, v_pages=16)
+args = _lib.PagedAttentionArgs(**common)
+args.struct_size = ctypes.sizeof(args)
+assert _lib.lib().pkda_paged_attention_workspace(ctypes.byref(args)) == 0
+_lib.call("pkda_paged_attention", args, 0)
+_lib.call("pkda_paged_append", _lib.PagedAppendArgs(**common), 0)
+print("done")
+"""
+    got = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and "done" in got.stdout, (got.returncode, got.stderr[-500:])
