@@ -166,15 +166,22 @@ def stage_alg_bytes(D: int, per_channel: bool = False) -> dict[str, int]:
     }
 
 
-def kernel_source_hash() -> str:
+def kernel_source_hash(serving: bool = False) -> str:
     """SHA-256 over the library's kernel sources and C ABI header (sorted by
-    name): what a committed counter summary was measured on."""
+    name): what a committed counter summary was measured on.  The serving
+    operators' sources, which the PKDA kernels do not read, have one of their
+    own, with the header they share."""
     import hashlib
 
     h = hashlib.sha256()
-    files = sorted((ROOT / "delta_feedback_experiment_amd" / "csrc").glob("*.hip"))
-    files += sorted((ROOT / "delta_feedback_experiment_amd" / "csrc").glob("*.h"))
-    files += sorted((ROOT / "include").glob("*.h"))
+    csrc, include = ROOT / "delta_feedback_experiment_amd" / "csrc", ROOT / "include"
+    if serving:
+        files = sorted((csrc / "serve").glob("*.hip")) + sorted((csrc / "serve").glob("*.h"))
+        files += sorted((include / "serve").glob("*.h")) + [csrc / "pkda_common.h"]
+    else:
+        files = sorted(csrc.glob("*.hip"))
+        files += sorted(csrc.glob("*.h"))
+        files += sorted(include.glob("*.h"))
     for f in files:
         h.update(f.name.encode())
         h.update(f.read_bytes())

@@ -930,7 +930,7 @@ Plan plan(AttnParams& p, bool packed) {
   // More than 32 rows a sequence go to 128-row tiles: 13 prompts take 87 us so,
   // and 238 as tiles of 32 rows; 64 sequences of 40 rows after 1,900 keys 81 and
   // 101.  Not where those tiles leave the card half empty: one prompt of 1,531
-  // tokens, 8/2 heads, is 98 of them (47 us) or 386 of 32 rows (36 us).
+  // tokens, 8/2 heads, is 98 of them (48 us) or 386 of 32 rows (36 us).
   p.key_rows = 32;
   r.row_tiles = packed ? tile_bound(N, S, group, kRowTile, true) : 0;
   if (packed && r.row_tiles * heads < kSlots / 2) p.key_rows = INT32_MAX;

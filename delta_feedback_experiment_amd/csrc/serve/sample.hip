@@ -28,8 +28,8 @@
 //
 // Measured, BF16, 256 rows of 131,072 normal logits times 3 (a row a compute
 // unit; 67 MB read once are 17 us, with all the noise 42): greedy 17 us, top-k 50
-// 29, top-k 200 and top-p 0.9 35, min-p 0.05 27, no filter 45, top-p 0.5 56, 0.9
-// 91, 0.99 108, top-k 5000 97; 4 rows of 50,304: 9 to 56.  What is left of a
+// 29 to 32 by its logits, top-k 200 and top-p 0.9 35, min-p 0.05 27, no filter 45,
+// top-p 0.5 53, 0.9 90, 0.99 109, top-k 5000 97; 4 rows of 50,304: 9 to 56.  What is left of a
 // top-p row is one exponential and one column addition a logit, then some 20
 // block-wide steps one after another.
 #include "pkda_common.h"
