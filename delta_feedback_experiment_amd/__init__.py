@@ -13,7 +13,10 @@ expansion runs inside the gate kernel, ``chunk_pkda(..., decay_up=...)``), and
 the slot-pool serving path that connects a cached prefill to the decode step
 (:mod:`.serve`).  For the trunk's attention layers a server finds the paged
 key/value cache and the attention over it (:mod:`.paged`), and for its last
-step the sampling of the next token (:mod:`.sample`).  Nothing here falls back to the CPU: without a HIP device and
+step the sampling of the next token (:mod:`.sample`); under load a cache of
+8-bit floats (:mod:`.paged_fp8`), attention of sequences that share a prefix
+(:mod:`.paged_prefix`) and the verification of drafted tokens (:mod:`.verify`).
+Nothing here falls back to the CPU: without a HIP device and
 the built library every operator raises.
 """
 
@@ -23,10 +26,14 @@ from .conv import pkda_qkv_conv
 from .norm_gate import pkda_norm_gate
 from .ops import pkda_recurrence
 from .paged import PagedKV, paged_append_, paged_attention
+from .paged_fp8 import PagedKVFP8, paged_append_fp8_, paged_attention_fp8
+from .paged_prefix import paged_prefix_attention
 from .pkda import fused_recurrent_pkda, pkda_decode_step_
 from .sample import sample_tokens
 from .serve import DecodePool, pkda_prefill_, pkda_qkv_conv_cached_
+from .verify import verify_tokens
 
-__all__ = ["DecodePool", "PagedKV", "chunk_pkda", "fused_recurrent_pkda", "paged_append_", "paged_attention",
-           "pkda_controls", "pkda_decode_step_", "pkda_norm_gate", "pkda_prefill_", "pkda_qkv_conv",
-           "pkda_qkv_conv_cached_", "pkda_recurrence", "sample_tokens"]
+__all__ = ["DecodePool", "PagedKV", "PagedKVFP8", "chunk_pkda", "fused_recurrent_pkda", "paged_append_",
+           "paged_append_fp8_", "paged_attention", "paged_attention_fp8", "paged_prefix_attention", "pkda_controls",
+           "pkda_decode_step_", "pkda_norm_gate", "pkda_prefill_", "pkda_qkv_conv", "pkda_qkv_conv_cached_",
+           "pkda_recurrence", "sample_tokens", "verify_tokens"]

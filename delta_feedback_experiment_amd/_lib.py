@@ -17,6 +17,7 @@ from .build import library_path
 
 PKDA_F32 = 0
 PKDA_BF16 = 1
+PKDA_CACHE_FP8 = 2
 GATE_LOG_HEAD = 0
 GATE_LOG_CHANNEL = 1
 GATE_RAW_CHANNEL = 2
@@ -26,7 +27,7 @@ STAGE_FWD_STATE = 2
 STAGE_BWD_STATE = 1
 STAGE_BWD_CHUNK = 2
 ABI_VERSION = 14
-SERVE_ABI_VERSION = 1
+SERVE_ABI_VERSION = 2
 
 
 class RecurrentArgs(ctypes.Structure):
@@ -148,6 +149,11 @@ _PAGED_COMMON = [
 ]
 
 
+_SCALES = [
+    ("k_scales", c_void_p), ("v_scales", c_void_p), ("k_scale_stride", c_int64), ("v_scale_stride", c_int64),
+]
+
+
 class PagedAppendArgs(ctypes.Structure):
     _fields_ = [("struct_size", c_int32), ("dtype", c_int32)] + _PAGED_COMMON + [
         ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
@@ -159,11 +165,27 @@ class PagedAppendArgs(ctypes.Structure):
     ]
 
 
+class PagedStoreArgs(ctypes.Structure):
+    _fields_ = PagedAppendArgs._fields_ + [
+        ("cache_dtype", c_int32), ("norm_dtype", c_int32), ("q_norm", c_void_p), ("k_norm", c_void_p), ("eps", c_float),
+    ] + _SCALES
+
+
 class PagedAttentionArgs(ctypes.Structure):
     _fields_ = [("struct_size", c_int32), ("dtype", c_int32)] + _PAGED_COMMON + [
         ("q", c_void_p), ("q_stride", c_int64), ("k_pages", c_void_p), ("v_pages", c_void_p),
         ("k_page_stride", c_int64), ("v_page_stride", c_int64), ("scale", c_float),
         ("o", c_void_p), ("lse", c_void_p), ("workspace", c_void_p),
+    ]
+
+
+class PagedAttentionFP8Args(ctypes.Structure):
+    _fields_ = PagedAttentionArgs._fields_ + _SCALES
+
+
+class PagedPrefixArgs(ctypes.Structure):
+    _fields_ = PagedAttentionArgs._fields_ + _SCALES + [
+        ("cu_groups", c_void_p), ("prefix_lens", c_void_p), ("num_groups", c_int32),
     ]
 
 
@@ -177,9 +199,20 @@ class SampleArgs(ctypes.Structure):
     ]
 
 
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_int32), ("dtype", c_int32), ("rows", c_int32), ("vocab", c_int32), ("num_seqs", c_int32),
+        ("logits", c_void_p), ("logits_stride", c_int64), ("draft_logits", c_void_p), ("draft_stride", c_int64),
+        ("drafts", c_void_p), ("uniform", c_void_p), ("noise", c_void_p), ("noise_stride", c_int64),
+        ("cu_seqlens", c_void_p), ("temperature", c_void_p), ("temperature_all", c_float),
+        ("tokens", c_void_p), ("accepted", c_void_p), ("workspace", c_void_p),
+    ]
+
+
 _ARG_KINDS = {0: RecurrentArgs, 1: GateArgs, 2: PrecondArgs, 3: ChunkFwdArgs, 4: ChunkBwdArgs, 5: QkvConvArgs,
               6: NormGateArgs, 7: ControlsArgs}
-_SERVE_ARG_KINDS = {0: PagedAppendArgs, 1: PagedAttentionArgs, 2: SampleArgs}
+_SERVE_ARG_KINDS = {0: PagedAppendArgs, 1: PagedAttentionArgs, 2: SampleArgs, 3: PagedStoreArgs,
+                    4: PagedAttentionFP8Args, 5: PagedPrefixArgs, 6: VerifyArgs}
 _LIB: ctypes.CDLL | None = None
 
 
@@ -233,7 +266,9 @@ def lib() -> ctypes.CDLL:
         ("pkda_norm_gate_fwd", NormGateArgs), ("pkda_norm_gate_bwd", NormGateArgs),
         ("pkda_controls_fwd", ControlsArgs), ("pkda_controls_bwd", ControlsArgs),
         ("pkda_paged_append", PagedAppendArgs), ("pkda_paged_attention", PagedAttentionArgs),
-        ("pkda_sample", SampleArgs),
+        ("pkda_sample", SampleArgs), ("pkda_paged_store", PagedStoreArgs),
+        ("pkda_paged_attention_fp8", PagedAttentionFP8Args), ("pkda_paged_prefix_attention", PagedPrefixArgs),
+        ("pkda_verify", VerifyArgs),
     ):
         fn = getattr(handle, name, None)
         if fn is not None:
@@ -250,8 +285,14 @@ def lib() -> ctypes.CDLL:
     handle.pkda_serve_abi_version.restype = c_int32
     handle.pkda_serve_args_size.restype = c_int64
     handle.pkda_serve_args_size.argtypes = [c_int32]
-    handle.pkda_paged_attention_workspace.restype = c_int64
-    handle.pkda_paged_attention_workspace.argtypes = [POINTER(PagedAttentionArgs)]
+    for name, struct in (
+        ("pkda_paged_attention_workspace", PagedAttentionArgs),
+        ("pkda_paged_attention_fp8_workspace", PagedAttentionFP8Args),
+        ("pkda_paged_prefix_workspace", PagedPrefixArgs), ("pkda_verify_workspace", VerifyArgs),
+    ):
+        fn = getattr(handle, name)
+        fn.restype = c_int64
+        fn.argtypes = [POINTER(struct)]
     if handle.pkda_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libpkda ABI {handle.pkda_abi_version()} != binding ABI {ABI_VERSION}")
     if handle.pkda_serve_abi_version() != SERVE_ABI_VERSION:

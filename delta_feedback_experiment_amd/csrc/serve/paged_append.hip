@@ -38,49 +38,6 @@ struct AppendParams {
   int slots;  // waves of a token
 };
 
-template <typename T> struct Vec8;  // eight channels
-template <> struct Vec8<bf16_t> {
-  uint4 r;
-  __device__ __forceinline__ void load(const bf16_t* p) { r = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void store(bf16_t* p) const { *reinterpret_cast<uint4*>(p) = r; }
-  __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float* x) const {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
-  __device__ __forceinline__ void set(const float* x) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = static_cast<uint32_t>(f32_to_bf16(x[2 * i])) | (static_cast<uint32_t>(f32_to_bf16(x[2 * i + 1])) << 16);
-    r = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-template <> struct Vec8<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = *reinterpret_cast<const float4*>(p);
-    b = *reinterpret_cast<const float4*>(p + 4);
-  }
-  __device__ __forceinline__ void store(float* p) const {
-    *reinterpret_cast<float4*>(p) = a;
-    *reinterpret_cast<float4*>(p + 4) = b;
-  }
-  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ void get(float* x) const {
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  }
-  __device__ __forceinline__ void set(const float* x) {
-    a = make_float4(x[0], x[1], x[2], x[3]);
-    b = make_float4(x[4], x[5], x[6], x[7]);
-  }
-};
-
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendParams p) {
   constexpr int L = D / 16;   // lanes of a head

@@ -32,8 +32,7 @@
 // top-p 0.5 53, 0.9 90, 0.99 109, top-k 5000 97; 4 rows of 50,304: 9 to 56.  What is left of a
 // top-p row is one exponential and one column addition a logit, then some 20
 // block-wide steps one after another.
-#include "pkda_common.h"
-#include "serve/pkda_serve_gfx950.h"
+#include "logits.h"
 
 namespace pkda {
 namespace {
@@ -43,7 +42,6 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kList = 1024;              // tokens of a sorted list: one a thread
 constexpr int kBins = 32, kFewBins = 8;  // of a round over the row, over a list: what LDS has room for
 constexpr int kCandidates = 27136;       // tokens of an unsorted list: likewise
-constexpr float kMaxFloat = 3.402823466e38f;
 constexpr uint32_t kMinKey = 0x00800000u;  // the key of -kMaxFloat
 
 struct SampleParams {
@@ -63,9 +61,6 @@ struct SampleParams {
   int vocab;
 };
 
-// A logit as the operator takes it: NaN as -inf (never taken), +inf as the
-// largest finite number.
-__device__ __forceinline__ float usable(float x) { return x > -INFINITY ? fminf(x, kMaxFloat) : -INFINITY; }
 // Order-preserving integer of a usable logit (-0 as +0); 0 for -inf.
 __device__ __forceinline__ uint32_t float_key(float x) {
   if (!(x > -INFINITY)) return 0;
@@ -81,37 +76,6 @@ __device__ __forceinline__ uint64_t order_key(float x, int i) {
 }
 __device__ __forceinline__ int key_index(uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
 __device__ __forceinline__ float key_logit(uint64_t key) { return key_float(static_cast<uint32_t>(key >> 32)); }
-
-// 16 bytes of a row that begins anywhere.
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef f32x4 f32x4_any __attribute__((aligned(4)));
-template <typename T> struct Logits;
-template <> struct Logits<float> {
-  static constexpr int N = 4;
-  static constexpr uint32_t none = 0xff800000u;  // -inf
-  __device__ __forceinline__ static float get(const u32x4& v, int j) { return __uint_as_float(v[j]); }
-  __device__ __forceinline__ static void clean(u32x4& v) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(usable(get(v, j)));
-  }
-};
-template <> struct Logits<bf16_t> {
-  static constexpr int N = 8;
-  static constexpr uint32_t none = 0xff80ff80u;
-  __device__ __forceinline__ static float get(const u32x4& v, int j) {
-    return __uint_as_float(j & 1 ? v[j / 2] & 0xffff0000u : v[j / 2] << 16);
-  }
-  // (the largest BF16 for +inf: kMaxFloat has no BF16 of its own)
-  __device__ __forceinline__ static void clean(u32x4& v) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = __float_as_uint(usable(get(v, 2 * j))), hi = __float_as_uint(usable(get(v, 2 * j + 1)));
-      v[j] = (lo >> 16) | (hi & 0xffff0000u);
-    }
-  }
-};
 
 // A row of logits and its noise.  odd: some logit is NaN or +inf, so that every
 // vector is cleaned as it is read.

@@ -35,6 +35,8 @@ from . import _lib, _registry
 from .pkda import _dtype_code, _on, _ptr, _require_cuda, _require_device, _stream
 
 HEAD_DIMS = (32, 64, 128)
+HEAD_DIMS_FP8 = (64, 128)
+SCALE_BLOCK = 32  # channels of one scale of a cache of 8-bit floats
 
 
 @dataclass
@@ -52,21 +54,25 @@ class PagedKV:
 
 
 def _check_cache(name: str, x: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seq_lens: Tensor,
-                 cu_seqlens: Tensor | None) -> None:
-    """The checks the two operators share; ``x`` is a token tensor."""
+                 cu_seqlens: Tensor | None, scales: tuple[Tensor, Tensor] | None = None) -> None:
+    """The checks the operators share; ``x`` is a token tensor, ``scales`` those of a cache of 8-bit floats."""
     shape, pages, dtype, lens = x.shape, k_pages.shape, x.dtype, seq_lens.shape
     if len(shape) != 3:
         raise ValueError(f"{name} [tokens, heads, head_dim] expected, got {tuple(shape)}")
     if len(pages) != 4 or pages != v_pages.shape:
         raise ValueError(f"k_pages {tuple(pages)} and v_pages {tuple(v_pages.shape)} must be one "
                          "[pages, page_size, kv_heads, head_dim] shape")
-    if dtype != k_pages.dtype or dtype != v_pages.dtype:
-        raise ValueError(f"{name} {dtype} and the pages {k_pages.dtype}, {v_pages.dtype} must share one dtype")
+    if scales is None:
+        if dtype != k_pages.dtype or dtype != v_pages.dtype:
+            raise ValueError(f"{name} {dtype} and the pages {k_pages.dtype}, {v_pages.dtype} must share one dtype")
+    elif k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"pages of 8-bit floats are float8_e4m3fn, not {k_pages.dtype}, {v_pages.dtype}")
     if dtype != torch.bfloat16 and dtype != torch.float32:
         raise ValueError(f"float32 or bfloat16 expected, not {dtype}")
-    _, R, H, D = pages
-    if shape[2] != D or D not in HEAD_DIMS:
-        raise ValueError(f"head_dim {shape[2]} of {name} and {D} of the pages: one of {HEAD_DIMS} expected")
+    P, R, H, D = pages
+    dims = HEAD_DIMS if scales is None else HEAD_DIMS_FP8
+    if shape[2] != D or D not in dims:
+        raise ValueError(f"head_dim {shape[2]} of {name} and {D} of the pages: one of {dims} expected")
     if R < 1 or H < 1:
         raise ValueError(f"pages {tuple(pages)} hold nothing")
     if seq_lens.dtype != torch.int32 or len(lens) != 1:
@@ -84,13 +90,21 @@ def _check_cache(name: str, x: Tensor, k_pages: Tensor, v_pages: Tensor, page_ta
         if (stride[3] != 1 or (stride[2] != D and H > 1) or (stride[1] != H * D and R > 1)
                 or not _aligned(t, stride[0])) and t.numel():
             raise ValueError("every page must be dense, in whole 16 bytes")
+    for t in scales or ():
+        B = D // SCALE_BLOCK
+        if t.dtype != torch.float8_e8m0fnu or tuple(t.shape) != (P, R, H, B):
+            raise ValueError(f"scales must be float8_e8m0fnu {(P, R, H, B)}, not {t.dtype} {tuple(t.shape)}")
+        stride = t.stride()
+        if (stride[3] != 1 or (stride[2] != B and H > 1) or (stride[1] != H * B and R > 1)
+                or not _aligned(t, stride[0], B)) and t.numel():
+            raise ValueError(f"every page's scales must be dense, in whole rows of {B} bytes")
 
 
-def _aligned(t: Tensor, stride: int) -> bool:
+def _aligned(t: Tensor, stride: int, to: int = 16) -> bool:
     # fake tensors have no address: the offset is what a view adds to its storage (a
     # compiler's trace has no offset either; the launch checks the address)
     offset = 0 if torch.compiler.is_compiling() else t.storage_offset()
-    return (stride | offset) * t.element_size() % 16 == 0
+    return (stride | offset) * t.element_size() % to == 0
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -145,6 +159,9 @@ def paged_append_(
     cos: Tensor | None = None,
     sin: Tensor | None = None,
     interleaved: bool = False,
+    q_norm: Tensor | None = None,
+    k_norm: Tensor | None = None,
+    eps: float = 1e-6,
     check_pages: bool = False,
 ) -> Tensor | None:
     """Store new keys and values in the cache; returns the rotated queries
@@ -162,9 +179,30 @@ def paged_append_(
     of ``q`` and ``k`` turn by their position's angles: pairs ``(c, c + rotary
     / 2)``, or ``(2c, 2c + 1)`` when ``interleaved``.  Without, they are
     copied.  Rows of the result whose token has no position are zeros.
+
+    With ``q_norm, k_norm`` (``[head_dim]``, FP32 or BF16, either alone too)
+    every head of ``q`` or ``k`` is first divided by its root mean square,
+    ``x (mean x^2 + eps)^(-1/2) weight``; norm and rotation are FP32, rounded
+    once.
     """
-    _require_device(k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, cos, sin)
+    _require_device(k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, cos, sin, q_norm, k_norm)
     _check_cache("k", k, k_pages, v_pages, page_table, seq_lens, cu_seqlens)
+    _check_append(k, v, k_pages, page_table, q, cos, sin, q_norm, k_norm)
+    if check_pages:
+        validate_pages(page_table, seq_lens, cu_seqlens, k.shape[0], k_pages.shape[0], k_pages.shape[1],
+                       appended=True)
+    if q_norm is None and k_norm is None:
+        out = _registry.launch(append_op, k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, cos, sin,
+                               bool(interleaved))
+    else:
+        out = _registry.launch(store_op, k, v, k_pages, v_pages, None, None, page_table, seq_lens, cu_seqlens, q, cos,
+                               sin, bool(interleaved), q_norm, k_norm, float(eps))
+    return None if q is None else out
+
+
+def _check_append(k: Tensor, v: Tensor, k_pages: Tensor, page_table: Tensor, q: Tensor | None, cos: Tensor | None,
+                  sin: Tensor | None, q_norm: Tensor | None, k_norm: Tensor | None) -> None:
+    """What an append checks beside the cache."""
     if v.shape != k.shape or v.dtype != k.dtype or k.shape[1] != k_pages.shape[2]:
         raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)} and pages of {k_pages.shape[2]} heads must match")
     if q is not None and (q.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype != k.dtype
@@ -180,12 +218,13 @@ def paged_append_(
             raise ValueError(f"rotary dim {2 * cos.shape[1]}: a multiple of 16 up to {k.shape[2]} expected")
         if cos.shape[0] < capacity:
             raise ValueError(f"cos and sin hold {cos.shape[0]} positions, a row of page_table {capacity}")
-    if check_pages:
-        validate_pages(page_table, seq_lens, cu_seqlens, k.shape[0], k_pages.shape[0], k_pages.shape[1],
-                       appended=True)
-    out = _registry.launch(append_op, k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, cos, sin,
-                           bool(interleaved))
-    return None if q is None else out
+    if q_norm is not None and q is None:
+        raise ValueError("q_norm without q")
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None and (tuple(w.shape) != (k.shape[2],) or w.dtype not in (torch.float32, torch.bfloat16)):
+            raise ValueError(f"{name} must be float32 or bfloat16 [{k.shape[2]}], not {w.dtype} {tuple(w.shape)}")
+    if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
+        raise ValueError(f"q_norm {q_norm.dtype} and k_norm {k_norm.dtype} must share one dtype")
 
 
 @_registry.device_op(
@@ -231,6 +270,61 @@ def _append_fake(k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, co
 _registry.register_fake(append_op, _append_fake)
 
 
+def _dense(t: Tensor | None) -> Tensor | None:
+    """A table of numbers as the kernels read it."""
+    return t if t is None or (t.is_contiguous() and _aligned(t, 0)) else t.clone(memory_format=torch.contiguous_format)
+
+
+@_registry.device_op(
+    "paged_store_(Tensor k, Tensor v, Tensor(a2!) k_pages, Tensor(a3!) v_pages, Tensor(a4!)? k_scales, "
+    "Tensor(a5!)? v_scales, Tensor page_table, Tensor seq_lens, Tensor? cu_seqlens, Tensor? q, Tensor? cos, "
+    "Tensor? sin, bool interleaved, Tensor? q_norm, Tensor? k_norm, float eps) -> Tensor")
+def store_op(
+    k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor | None, v_scales: Tensor | None,
+    page_table: Tensor, seq_lens: Tensor, cu_seqlens: Tensor | None, q: Tensor | None, cos: Tensor | None,
+    sin: Tensor | None, interleaved: bool, q_norm: Tensor | None, k_norm: Tensor | None, eps: float,
+) -> Tensor:
+    """The launch of an append with norms, or into a cache of 8-bit floats
+    (arguments checked by :func:`paged_append_` and
+    :func:`.paged_fp8.paged_append_fp8_`); returns the queries as ``append_op``."""
+    _require_cuda(k, v, k_pages, v_pages, k_scales, v_scales, page_table, seq_lens, cu_seqlens, q, cos, sin, q_norm,
+                  k_norm)
+    k, v = _rows(k), _rows(v)
+    q = None if q is None else _rows(q)
+    q_out = k.new_empty((0,) if q is None else q.shape)
+    cos, sin, q_norm, k_norm = _dense(cos), _dense(sin), _dense(q_norm), _dense(k_norm)
+    page_table, seq_lens = _ints(page_table), _ints(seq_lens)
+    cu_seqlens = None if cu_seqlens is None else _ints(cu_seqlens)
+    weight = k_norm if q_norm is None else q_norm
+    args = _lib.PagedStoreArgs(
+        dtype=_dtype_code(k), num_seqs=seq_lens.shape[0], num_tokens=k.shape[0],
+        q_heads=0 if q is None else q.shape[1], kv_heads=k.shape[1], head_dim=k.shape[2],
+        page_size=k_pages.shape[1], max_pages=page_table.shape[1], num_pages=k_pages.shape[0],
+        table_stride=page_table.stride(0), cu_seqlens=_ptr(cu_seqlens), seq_lens=_ptr(seq_lens),
+        page_table=_ptr(page_table), q=_ptr(q), k=_ptr(k), v=_ptr(v),
+        q_stride=0 if q is None else q.stride(0), k_stride=k.stride(0), v_stride=v.stride(0),
+        q_out=_ptr(q_out), k_pages=_ptr(k_pages), v_pages=_ptr(v_pages),
+        k_page_stride=k_pages.stride(0), v_page_stride=v_pages.stride(0), cos=_ptr(cos), sin=_ptr(sin),
+        rotary_dim=0 if cos is None else 2 * cos.shape[1], interleaved=int(interleaved),
+        rope_rows=0 if cos is None else cos.shape[0],
+        cache_dtype=_dtype_code(k) if k_scales is None else _lib.PKDA_CACHE_FP8,
+        norm_dtype=0 if weight is None else _dtype_code(weight), q_norm=_ptr(q_norm), k_norm=_ptr(k_norm), eps=eps,
+    )
+    if k_scales is not None:
+        args.k_scales, args.v_scales = _ptr(k_scales), _ptr(v_scales)
+        args.k_scale_stride, args.v_scale_stride = k_scales.stride(0), v_scales.stride(0)
+    with _on(k.device):
+        _lib.call("pkda_paged_store", args, _stream(k.device))
+    return q_out
+
+
+def _store_fake(k, v, k_pages, v_pages, k_scales, v_scales, page_table, seq_lens, cu_seqlens, q, *rest):
+    return k.new_empty((0,) if q is None else q.shape)
+
+
+_registry.register_fake(store_op, _store_fake)
+
+
 def paged_attention(
     q: Tensor,
     k_pages: Tensor,
@@ -274,25 +368,36 @@ def attention_op(
 ) -> tuple[Tensor, Tensor]:
     """The attention's launches (arguments checked by :func:`paged_attention`)."""
     device = _require_cuda(q, k_pages, v_pages, page_table, seq_lens, cu_seqlens)
+    return _attend(_lib.PagedAttentionArgs, "pkda_paged_attention", "pkda_paged_attention_workspace", device, q, k_pages,
+                   v_pages, None, None, page_table, seq_lens, cu_seqlens, scale)
+
+
+def _attend(struct, entry: str, sizes: str, device: torch.device, q: Tensor, k_pages: Tensor, v_pages: Tensor,
+            k_scales: Tensor | None, v_scales: Tensor | None, page_table: Tensor, seq_lens: Tensor,
+            cu_seqlens: Tensor | None, scale: float, **more) -> tuple[Tensor, Tensor]:
+    """The call of one of the attention entry points."""
     q = _rows(q)
     page_table, seq_lens = _ints(page_table), _ints(seq_lens)
     cu_seqlens = None if cu_seqlens is None else _ints(cu_seqlens)
     N, Hq, D = q.shape
     o = torch.empty(N, Hq, D, dtype=q.dtype, device=device)
     lse = torch.empty(N, Hq, dtype=torch.float32, device=device)
-    args = _lib.PagedAttentionArgs(
+    args = struct(
         dtype=_dtype_code(q), num_seqs=seq_lens.shape[0], num_tokens=N, q_heads=Hq, kv_heads=k_pages.shape[2],
         head_dim=D, page_size=k_pages.shape[1], max_pages=page_table.shape[1], num_pages=k_pages.shape[0],
         table_stride=page_table.stride(0), cu_seqlens=_ptr(cu_seqlens), seq_lens=_ptr(seq_lens),
         page_table=_ptr(page_table), q=_ptr(q), q_stride=q.stride(0), k_pages=_ptr(k_pages), v_pages=_ptr(v_pages),
-        k_page_stride=k_pages.stride(0), v_page_stride=v_pages.stride(0), scale=scale, o=_ptr(o), lse=_ptr(lse),
+        k_page_stride=k_pages.stride(0), v_page_stride=v_pages.stride(0), scale=scale, o=_ptr(o), lse=_ptr(lse), **more,
     )
+    if k_scales is not None:
+        args.k_scales, args.v_scales = _ptr(k_scales), _ptr(v_scales)
+        args.k_scale_stride, args.v_scale_stride = k_scales.stride(0), v_scales.stride(0)
     args.struct_size = ctypes.sizeof(args)
-    floats = _lib.lib().pkda_paged_attention_workspace(ctypes.byref(args))
+    floats = getattr(_lib.lib(), sizes)(ctypes.byref(args))
     workspace = torch.empty(floats, dtype=torch.float32, device=device) if floats > 0 else None
     args.workspace = _ptr(workspace)
     with _on(device):
-        _lib.call("pkda_paged_attention", args, _stream(device))
+        _lib.call(entry, args, _stream(device))
     return o, lse
 
 
