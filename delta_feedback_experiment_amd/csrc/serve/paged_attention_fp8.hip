@@ -8,6 +8,12 @@
 // Up to 32 rows a sequence a lane converts its key's chunks in registers, the
 // keys' for the first product and the values' on their way to LDS; more rows
 // convert what they stage, so that a number is converted once for 128 rows.
+//
+// What bounds it, in BF16 with heads of 128 (a 4 GiB copy runs at 4.55 TB/s).
+// Decode, 256 sequences of 325 to 4,875 keys, 32/8 heads: 288 us, 4.95 TB/s of codes
+// and scales (547 us over a BF16 cache).  4 sequences of 700 keys: 5.9 us and 3.6 for
+// the join, a trip to memory after the other.  2,048 tokens after 14,336: 600 us, 857
+// TFLOP/s, what the same takes over a BF16 cache: softmax beside products.
 #include "paged_attention.h"
 
 namespace pkda {

@@ -26,16 +26,34 @@ struct PrefixPlan {
 // The two parts' forms and splits, from what the host knows.
 inline PrefixPlan prefix_plan(AttnParams& shared, AttnParams& own) {
   PrefixPlan r;
-  AttnParams groups = shared;  // to the rules a group is a sequence
-  groups.s.num_seqs = shared.num_groups;
-  r.shared = plan(groups, true);
-  shared.splits = groups.splits < kMaxSplits / 2 ? groups.splits : kMaxSplits / 2;
-  shared.min_chunk = groups.min_chunk;
-  shared.key_rows = groups.key_rows;
+  const int64_t group = shared.group.d, N = shared.s.num_tokens, G = shared.num_groups, heads = shared.kv_heads;
+  // Groups of more than 32 rows are tiles of 128, however few: their keys are split
+  // over one workgroup a compute unit, so that the own parts' workgroups, which wait
+  // for memory, run beside them.  64 sequences of 300 keys behind 16,384, 32/8 heads:
+  // 57 us with splits for 256 workgroups, 60 with 384, 64 with 512 (and 103 where the
+  // own part has four splits); of at least 256 keys, which 32 sequences of 5 tokens
+  // behind 7,000 take 34 us with, 512 keys 34, 1,024 37, 6 groups of 16 behind 2,500
+  // 28, 30 and 42.
+  shared.key_rows = 32;
+  r.shared.row_tiles = tile_bound(N, G, group, kRowTile, true);
+  r.shared.key_tiles = G;
+  const int64_t per_group = G > 0 ? (N * group + G - 1) / G : 0;
+  const int64_t tiles = per_group > 32 ? G * ((per_group + kRowTile - 1) / kRowTile) : G;
+  shared.min_chunk = per_group > 32 ? 256 : kMinChunk;
+  int64_t want = kSlots / 2 / (tiles * heads > 0 ? tiles * heads : 1);
+  const int64_t cap = ((int64_t)shared.s.max_pages * shared.s.page_size + shared.min_chunk - 1) / shared.min_chunk;
+  if (want > cap) want = cap;
+  if (want > kMaxSplits / 2) want = kMaxSplits / 2;
+  shared.splits = want < 1 ? 1 : (int)want;
   shared.whole = 0;
-  if (groups.key_rows == 32) r.shared.key_tiles = shared.num_groups;
   r.own = plan(own, own.s.cu != nullptr);
-  if (own.splits > kMaxSplits / 2) own.splits = kMaxSplits / 2;
+  // What the sequences hold by themselves is not known here, and seldom long: no more
+  // workgroups than the card holds.  The same 64 sequences take 57 us, with four times
+  // as many 76, the 6 groups 28 and 32; 8 sequences of 3,000 behind 2,048 31 and 37.
+  const int64_t items = (r.own.row_tiles + r.own.key_tiles) * heads;
+  int64_t most = kSlots / (items > 0 ? items : 1);
+  most = most < 1 ? 1 : most < kMaxSplits / 2 ? most : kMaxSplits / 2;
+  if (own.splits > most) own.splits = (int)most;
   return r;
 }
 
@@ -55,10 +73,12 @@ int launch_prefix(AttnParams shared, AttnParams own, hipStream_t s) {
   own.part_o = shared.part_o + shared.splits * rows * G::D;
   own.part_ml = shared.part_ml + shared.splits * rows * 2;
   const dim3 grid((unsigned)blocks), block(kThreads);
-  if (own.s.page_size % (64 / G::SC) == 0)
-    hipLaunchKernelGGL((paged_prefix_kernel<G, true>), grid, block, 0, s, shared, own, (unsigned)first);
-  else
-    hipLaunchKernelGGL((paged_prefix_kernel<G, false>), grid, block, 0, s, shared, own, (unsigned)first);
+  const bool few = !own.s.cu && own.group.d <= kFewRows, whole = own.s.page_size % (64 / G::SC) == 0;
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, shared, own, (unsigned)first); };
+  if (few && whole) launch(paged_prefix_kernel<G, true, true>);
+  else if (few) launch(paged_prefix_kernel<G, false, true>);
+  else if (whole) launch(paged_prefix_kernel<G, true, false>);
+  else launch(paged_prefix_kernel<G, false, false>);
   if (int st = launch_status(what)) return st;
   return launch_join<G, true>(shared, own, s, what);
 }

@@ -15,6 +15,10 @@
 // two vectors of eight that rotate into each other (or neighbours).  A head's sum
 // of squares is its D / 16 lanes'; a block's maximum too, block by block, since a
 // lane's two vectors lie in blocks that depend on the rotated channels.
+//
+// Measured (BF16, heads of 128, every channel turned, norms): 11,180 tokens of 16 + 2
+// x 4 heads in 13 sequences into 8-bit floats, 87 MB of least traffic: 20.7 us; into
+// BF16, 94 MB: 20.3 us, 4.6 TB/s.  4 tokens: 3.7 us.
 #include "paged_common.h"
 
 namespace pkda {

@@ -11,11 +11,15 @@
 // piece's maximum m and sum of 2^((l - m) c), c = log2 e / T: whether a row is
 // reached is known only after those before it, and reading it anyway costs less
 // than a trip to memory per draft.  In the second, every workgroup of a sequence
-// joins the pieces of its rows, four rows at a time, until a draft is not accepted,
-// and scans its part of that one row; the last to finish joins the parts (the
-// lowest index of the highest score does not depend on their order).
+// joins the pieces of its rows, eight rows at a time, until a draft is not accepted,
+// and scans its part of that one row; the parts' best, the lowest index of the
+// highest score, does not depend on their order.
 //
-// Sums are FP32 within a piece of a few thousand logits, FP64 over pieces.
+// Sums are FP32: a thread's, the wave's in pairs, the pieces' in pairs.
+//
+// Measured, BF16: 64 sequences of up to 5 drafts, 131,072 tokens, 322 rows and 258 of
+// the drafts': 33 us for the sums (152 MB, 4.6 TB/s) and 21 for the picks (50 MB, behind
+// three trips to memory one after another).
 #include "logits.h"
 #include "paged_common.h"
 
@@ -32,11 +36,18 @@ struct Sum {  // a piece of a row
   float m, s;      // maximum and sum of the target's
   float dm, ds;    // and of the draft's
   int first;       // lowest index of the target's maximum
-  int pad[3];
+  int drafted;     // in a row's first piece: the row's draft, -1 for none that can be taken,
+  float l, dl;     // and its logits
 };
+// A score and its token as one number, so that the larger is the better: the
+// score's order, then the lower index.  0: none.
 struct Best {
-  float score;
-  int index;
+  uint64_t key;
+  __device__ __forceinline__ static uint64_t of(float score, int index) {
+    const uint32_t b = __float_as_uint(score + 0.f);
+    return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~index;
+  }
+  __device__ __forceinline__ int index() const { return (int)~(uint32_t)key; }
 };
 
 struct VerifyParams {
@@ -51,9 +62,12 @@ struct VerifyParams {
   int parts;   // of the last row, in the second
   int32_t *tokens, *accepted;
   Sum* sums;   // [rows][pieces]
-  Best* best;  // [num_seqs][parts]
-  int32_t* done;  // [num_seqs] parts that are done
+  uint64_t* best;  // [num_seqs] of the parts that are done
+  int32_t* done;   // [num_seqs] how many those are
 };
+
+template <typename T>
+__device__ __forceinline__ float one_logit(const T* l, int i) { return usable(io<T>::load(l + i)); }
 
 __device__ __forceinline__ int row_bound(const VerifyParams& p, int n) {
   return n == 0 ? 0 : clamp_int(p.cu[n], 0, p.rows);
@@ -147,7 +161,10 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyParams p) {
   __shared__ int s_first[kWaves];
   const int piece = blockIdx.x % p.pieces, row = blockIdx.x / p.pieces, tid = threadIdx.x;
   if (piece == 0)
-    for (int64_t i = (int64_t)row * kThreads + tid; i < p.num_seqs; i += (int64_t)p.rows * kThreads) p.done[i] = 0;
+    for (int64_t i = (int64_t)row * kThreads + tid; i < p.num_seqs; i += (int64_t)p.rows * kThreads) {
+      p.best[i] = 0;
+      p.done[i] = 0;
+    }
   const int n = wave_upper(p.num_seqs, row, [&](int i) -> int64_t { return row_bound(p, i); });
   if (n >= p.num_seqs) {  // a row of no sequence
     if (piece == 0 && tid == 0) p.tokens[row] = -1;
@@ -159,6 +176,18 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyParams p) {
   // the last row's draft, and a greedy row's draft logits, are not asked for
   const T* d = p.draft && !greedy && row + 1 < row_bound(p, n + 1) ? static_cast<const T*>(p.draft) + row * p.draft_stride : nullptr;
   const int vectors = (p.vocab + L::N - 1) / L::N, chunks = (vectors + kThreads * U - 1) / (kThreads * U);
+  // the draft's own logits, while the row's are on their way
+  Sum r;
+  r.drafted = -1;
+  r.l = r.dl = -INFINITY;
+  if (piece == 0 && tid == 0) {
+    const int i = p.drafts[row];
+    if ((unsigned)i < (unsigned)p.vocab) {
+      r.drafted = i;
+      r.l = one_logit(l, i);
+      if (d) r.dl = one_logit(d, i);
+    }
+  }
   float m = -INFINITY, s = 0.f, dm = -INFINITY, ds = 0.f;
   int first = INT32_MAX;
   for (int k = piece; k < chunks; k += p.pieces) {
@@ -218,7 +247,6 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyParams p) {
     if (d) block_sum(dm, ds, c, s_sum[1]);
   }
   if (tid == 0) {
-    Sum r;
     r.m = m; r.s = s; r.dm = dm; r.ds = ds; r.first = first;
     p.sums[(int64_t)row * p.pieces + piece] = r;
   }
@@ -228,58 +256,66 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyParams p) {
 // The drafts in turn, and the next token.
 // ---------------------------------------------------------------------------
 struct RowSum {
-  float m, dm;
-  double s, ds;
+  float m, s, dm, ds;
   int first;
 };
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-  return x;
+// f over the wave's x, every lane getting it.
+template <typename V, typename F>
+__device__ __forceinline__ V wave_all(V x, F f) {
+  const auto moved = [&](auto move) { return __builtin_bit_cast(V, move(__builtin_bit_cast(int, x))); };
+  x = f(x, moved([](int i) { return __builtin_amdgcn_update_dpp(0, i, 0xB1, 0xF, 0xF, false); }));   // quad [1,0,3,2]
+  x = f(x, moved([](int i) { return __builtin_amdgcn_update_dpp(0, i, 0x4E, 0xF, 0xF, false); }));   // quad [2,3,0,1]
+  x = f(x, moved([](int i) { return __builtin_amdgcn_update_dpp(0, i, 0x141, 0xF, 0xF, false); }));  // half-row mirror
+  x = f(x, moved([](int i) { return __builtin_amdgcn_update_dpp(0, i, 0x140, 0xF, 0xF, false); }));  // row mirror
+  int i = __builtin_bit_cast(int, x);
+  auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+  x = f(__builtin_bit_cast(V, (int)r[0]), __builtin_bit_cast(V, (int)r[1]));
+  i = __builtin_bit_cast(int, x);
+  r = __builtin_amdgcn_permlane32_swap(i, i, false, false);
+  return f(__builtin_bit_cast(V, (int)r[0]), __builtin_bit_cast(V, (int)r[1]));
 }
-__device__ __forceinline__ double wave_total(double x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+__device__ __forceinline__ float wave_max(float x) {
+  return wave_all(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_total(float x) {
+  return wave_all(x, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ int wave_min(int x) {
+  return wave_all(x, [](int a, int b) { return min(a, b); });
+}
+// A row's piece of this lane.
+__device__ __forceinline__ Sum lane_piece(const VerifyParams& p, int row) {
+  const int lane = threadIdx.x & 63;
+  Sum x;
+  x.m = x.dm = x.l = x.dl = -INFINITY;
+  x.s = x.ds = 0.f;
+  x.first = INT32_MAX;
+  x.drafted = -1;
+  if (lane < p.pieces) x = p.sums[(int64_t)row * p.pieces + lane];
   return x;
 }
 // A row's pieces joined, by a wave.
-__device__ __forceinline__ RowSum row_sum(const VerifyParams& p, int row, float c) {
-  const int lane = threadIdx.x & 63;
-  Sum x;
-  x.m = x.dm = -INFINITY;
-  x.s = x.ds = 0.f;
-  x.first = INT32_MAX;
-  if (lane < p.pieces) x = p.sums[(int64_t)row * p.pieces + lane];
+__device__ __forceinline__ RowSum row_sum(const Sum& x, float c) {
   RowSum r;
   r.m = wave_max(x.m);
   r.dm = wave_max(x.dm);
-  r.s = wave_total((double)x.s * carried(x.m, r.m, c));
-  r.ds = wave_total((double)x.ds * carried(x.dm, r.dm, c));
-  int first = x.m == r.m ? x.first : INT32_MAX;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) first = min(first, __shfl_xor(first, o));
-  r.first = first;
+  r.s = wave_total(x.s * carried(x.m, r.m, c));
+  r.ds = wave_total(x.ds * carried(x.dm, r.dm, c));
+  r.first = wave_min(x.m == r.m ? x.first : INT32_MAX);
   return r;
-}
-template <typename T>
-__device__ __forceinline__ float one_logit(const T* l, int i) { return usable(io<T>::load(l + i)); }
-
-__device__ __forceinline__ void take(Best& b, float score, int index) {
-  if (score > b.score || (score == b.score && index < b.index)) b = {score, index};
 }
 __device__ __forceinline__ Best block_best(Best b, Best (&lds)[kWaves]) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) {
-    const float score = __shfl_xor(b.score, o);
-    const int index = __shfl_xor(b.index, o);
-    take(b, score, index);
+    const uint64_t other = __shfl_xor((unsigned long long)b.key, o);
+    b.key = max(b.key, other);
   }
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = b;
   __syncthreads();
   b = lds[0];
 #pragma unroll
-  for (int i = 1; i < kWaves; ++i) take(b, lds[i].score, lds[i].index);
+  for (int i = 1; i < kWaves; ++i) b.key = max(b.key, lds[i].key);
   return b;
 }
 
@@ -291,6 +327,13 @@ __device__ __forceinline__ float difference(float a, float b, float q) {
   return p - q;
 }
 
+// ln x for x > 0 on the hardware log2, which takes no denormal numbers.
+__device__ __forceinline__ float log_of(float x) {
+  const bool small = x < 0x1p-96f;
+  const float l = __builtin_amdgcn_logf(small ? x * 0x1p64f : x);
+  return (small ? l - 64.f : l) * 0.693147180559945309f;
+}
+
 // The scores of a row's vectors part, part + parts, ... (in workgroups).  left: of
 // what p has more than q; otherwise of p but for `without`.
 template <typename T>
@@ -298,50 +341,62 @@ __device__ __forceinline__ Best scan_row(const VerifyParams& p, const T* l, cons
                                          const RowSum& r, bool left, int without, int part, int parts) {
   using L = Logits<T>;
   const int vectors = (p.vocab + L::N - 1) / L::N;
-  const float inv_t = fminf(1.f / t, kMaxFloat);
-  const float ps = (float)(1.0 / r.s), qs = r.ds > 0.0 ? (float)(1.0 / r.ds) : 0.f;
+  const float inv_t = fminf(1.f / t, kMaxFloat), c = exponent_factor(t);
+  const float ps = 1.f / r.s, qs = r.ds > 0.f ? 1.f / r.ds : 0.f;
   // x / T, the product's rounding made good where T is no power of two
   const auto over_t = [&](float x) {
     const float y = x * inv_t, e = __builtin_fmaf(-y, t, x);
     return fabsf(e) < INFINITY ? __builtin_fmaf(e, inv_t, y) : y;
   };
-  Best b = {-INFINITY, INT32_MAX};
-  for (int v = part * kThreads + threadIdx.x; v < vectors; v += parts * kThreads) {
-    u32x4 x = row_vector<T>(l, v, p.vocab), y = u32x4{L::none, L::none, L::none, L::none};
-    if (left) y = row_vector<T>(d, v, p.vocab);
-    float g[L::N];
+  float best = 0.f;
+  int index = -1;
+  constexpr int U = kVectors, NV = L::N / 4;
+  for (int v0 = part * kThreads + threadIdx.x; v0 < vectors; v0 += U * parts * kThreads) {
+    u32x4 x[U], y[U], g[U][NV];
 #pragma unroll
-    for (int j = 0; j < L::N; j += 4) {
-      const u32x4 a = row_vector<float>(noise, v * (L::N / 4) + j / 4, p.vocab);
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + u * parts * kThreads;
+      x[u] = y[u] = u32x4{L::none, L::none, L::none, L::none};
+      if (v >= vectors) continue;
+      x[u] = row_vector<T>(l, v, p.vocab);
+      if (left) y[u] = row_vector<T>(d, v, p.vocab);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) g[j + i] = __uint_as_float(a[i]);
+      for (int j = 0; j < NV; ++j) g[u][j] = row_vector<float>(noise, v * NV + j, p.vocab);
     }
-    L::clean(x);
-    L::clean(y);
 #pragma unroll
-    for (int j = 0; j < L::N; ++j) {
-      const int i = v * L::N + j;
-      const float lx = L::get(x, j);
-      if (!(lx > -INFINITY) || i == without) continue;
-      const float z = over_t(fmaxf(lx - r.m, -kMaxFloat));
-      float score = z;
-      if (left) {
-        const float ly = L::get(y, j);
-        const float q = ly > -INFINITY ? __builtin_amdgcn_exp2f(over_t(fmaxf(ly - r.dm, -kMaxFloat)) * kLog2e) * qs : 0.f;
-        const float rest = difference(__builtin_amdgcn_exp2f(z * kLog2e), ps, q);
-        if (!(rest > 0.f)) continue;
-        score = logf(rest);
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int j = 0; j < L::N; ++j) {
+        const int i = (v0 + u * parts * kThreads) * L::N + j;
+        const float lx = L::get(x[u], j);
+        bool in = lx > -INFINITY && i != without;
+        const float above = fmaxf(fminf(lx, r.m) - r.m, -kMaxFloat);  // (+inf is the row's maximum)
+        float score;
+        if (left) {
+          const float ly = L::get(y[u], j);
+          const float q = ly > -INFINITY ? __builtin_amdgcn_exp2f(fmaxf(fminf(ly, r.dm) - r.dm, -kMaxFloat) * c) * qs : 0.f;
+          const float rest = difference(__builtin_amdgcn_exp2f(above * c), ps, q);
+          in = in && rest > 0.f;
+          score = log_of(rest);
+        } else {
+          score = over_t(above);
+        }
+        score += __uint_as_float(g[u][j / 4][j % 4]);
+        if (in && (score > best || (index < 0 && score == score))) {  // (a thread's indices rise)
+          best = score;
+          index = i;
+        }
       }
-      take(b, score + g[j], i);
     }
   }
-  return b;
+  return {index < 0 ? 0 : Best::of(best, index)};
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyParams p) {
-  __shared__ RowSum s_row[kWaves];
-  __shared__ int s_stop[kWaves];
+  constexpr int kRows = 2;  // of a wave at a time
+  __shared__ RowSum s_row[kRows * kWaves];
+  __shared__ int s_stop[kRows * kWaves];
   __shared__ Best s_best[kWaves];
   __shared__ int s_last;
   const int part = blockIdx.x % p.parts, n = blockIdx.x / p.parts, tid = threadIdx.x;
@@ -353,40 +408,45 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyParams p) {
   }
   const float t = temperature_of(p, n), c = exponent_factor(t);
   const bool greedy = t <= 0.f;
+  const T* logits = static_cast<const T*>(p.logits);
+  const T* draft = static_cast<const T*>(p.draft);
   RowSum r;
   int stop = count - 1;
-  for (int j0 = 0; j0 < count; j0 += kWaves) {
-    const int j = j0 + w;
-    if (j < count) {
-      const int row = first + j;
-      const RowSum x = row_sum(p, row, c);
-      bool taken = false;
-      if (j + 1 < count) {
-        const int d = p.drafts[row];
-        if ((unsigned)d < (unsigned)p.vocab) {
+  for (int j0 = 0; j0 < count; j0 += kRows * kWaves) {
+    // everything of a wave's rows is asked for before any of it is waited for
+    Sum x[kRows];
+    float u[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int row = first + min(j0 + i * kWaves + w, count - 1);
+      u[i] = p.uniform[row];
+      x[i] = lane_piece(p, row);
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int j = j0 + i * kWaves + w;
+      const RowSum y = row_sum(x[i], c);
+      if ((tid & 63) == 0) {  // whose piece is the row's first
+        const Sum& z = x[i];
+        bool taken = false;
+        if (j + 1 < count && z.drafted >= 0) {
           if (greedy) {
-            taken = d == x.first;
+            taken = z.drafted == y.first;
           } else {
-            const float lp = one_logit(static_cast<const T*>(p.logits) + row * p.logits_stride, d);
-            const double pd = lp > -INFINITY && x.s > 0.0 ? (double)carried(lp, x.m, c) / x.s : 0.0;
-            double qd = 1.0;
-            if (p.draft) {
-              const float lq = one_logit(static_cast<const T*>(p.draft) + row * p.draft_stride, d);
-              qd = lq > -INFINITY && x.ds > 0.0 ? (double)carried(lq, x.dm, c) / x.ds : 0.0;
-            }
-            taken = (double)p.uniform[row] * qd < pd;
+            const float pd = z.l > -INFINITY && y.s > 0.f ? carried(z.l, y.m, c) / y.s : 0.f;
+            const float qd = !draft ? 1.f : z.dl > -INFINITY && y.ds > 0.f ? carried(z.dl, y.dm, c) / y.ds : 0.f;
+            taken = u[i] * qd < pd;
           }
         }
-      }
-      if ((tid & 63) == 0) {
-        s_row[w] = x;
-        s_stop[w] = !taken;
+        s_row[i * kWaves + w] = y;
+        s_stop[i * kWaves + w] = j < count && !taken;
       }
     }
     __syncthreads();
     int at = -1;
-    for (int i = kWaves - 1; i >= 0; --i)
-      if (j0 + i < count && s_stop[i]) at = i;
+#pragma unroll
+    for (int i = kRows * kWaves - 1; i >= 0; --i)
+      if (s_stop[i]) at = i;
     if (at >= 0) {
       r = s_row[at];
       stop = j0 + at;
@@ -399,37 +459,31 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyParams p) {
   bool last = part == 0;  // whether this workgroup writes the result
   if (greedy) {
     token = r.first == INT32_MAX ? -1 : r.first;
-  } else if (r.s > 0.0) {
-    const T* l = static_cast<const T*>(p.logits) + row * p.logits_stride;
-    const T* d = p.draft ? static_cast<const T*>(p.draft) + row * p.draft_stride : nullptr;
+  } else if (r.s > 0.f) {
+    const T* l = logits + row * p.logits_stride;
+    const T* q = draft ? draft + row * p.draft_stride : nullptr;
     const float* noise = p.noise + n * p.noise_stride;
     const bool rejected = stop + 1 < count;
-    const bool left = rejected && d;
-    const int without = rejected && !d ? p.drafts[row] : -1;
-    Best b = scan_row<T>(p, l, d, noise, t, r, left, without, part, p.parts);
-    b = block_best(b, s_best);
+    const bool left = rejected && q;
+    const int without = rejected && !q ? p.drafts[row] : -1;
+    Best b = block_best(scan_row<T>(p, l, q, noise, t, r, left, without, part, p.parts), s_best);
     if (p.parts > 1) {
+      // The parts' best by one atomic maximum: nothing but atomics passes between
+      // the workgroups, so that none has to write its cache back, and the count
+      // goes out when the maximum has come back.
       if (tid == 0) {
-        Best* out = p.best + (int64_t)n * p.parts + part;
-        __hip_atomic_store(&out->score, b.score, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(&out->index, b.index, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = __hip_atomic_fetch_add(p.done + n, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == p.parts - 1;
+        __hip_atomic_fetch_max(p.best + n, b.key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        s_last = __hip_atomic_fetch_add(p.done + n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.parts - 1;
       }
       __syncthreads();
       last = s_last;
       if (!last) return;
-      b = {-INFINITY, INT32_MAX};
-      for (int i = tid; i < p.parts; i += kThreads) {
-        Best* in = p.best + (int64_t)n * p.parts + i;
-        take(b, __hip_atomic_load(&in->score, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
-             __hip_atomic_load(&in->index, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-      }
-      b = block_best(b, s_best);
+      b.key = __hip_atomic_load(p.best + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     // nothing of p is left: p itself, by this workgroup alone
-    if (b.index == INT32_MAX && rejected)
-      b = block_best(scan_row<T>(p, l, d, noise, t, r, false, -1, 0, 1), s_best);
-    token = b.index == INT32_MAX ? -1 : b.index;
+    if (b.key == 0 && rejected) b = block_best(scan_row<T>(p, l, q, noise, t, r, false, -1, 0, 1), s_best);
+    token = b.key == 0 ? -1 : b.index();
   }
   if (!last) return;
   for (int j = tid; j < count; j += kThreads) p.tokens[first + j] = j < stop ? p.drafts[first + j] : j == stop ? token : -1;
@@ -440,17 +494,20 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyParams p) {
 // card, none with less than a vector a thread.
 void verify_plan(VerifyParams& p, int dtype) {
   const int64_t n = dtype == PKDA_BF16 ? 8 : 4, vectors = (p.vocab + n - 1) / n;
-  const auto pieces = [&](int64_t rows, int64_t each) {
-    int64_t want = (4096 + rows - 1) / (rows > 0 ? rows : 1);
+  const auto pieces = [&](int64_t rows, int64_t each, int64_t blocks) {
+    int64_t want = (blocks + rows - 1) / (rows > 0 ? rows : 1);
     const int64_t cap = (vectors + each - 1) / each;
     want = want < cap ? want : cap;
     return (int)(want < 1 ? 1 : want < kMaxPieces ? want : kMaxPieces);
   };
-  p.pieces = pieces(p.rows, kThreads * kVectors);
-  p.parts = pieces(p.num_seqs, kThreads);
+  // A part's way to its row is some trips to memory, however little it then scans:
+  // 64 sequences of 131,072 tokens, 64 parts each 59 us, 16 parts 55, 8 parts 60 (in
+  // all); 32 of 50,304 31, 27 and 25 with 50, 32 and 16.
+  p.pieces = pieces(p.rows, kThreads * kVectors, 4096);
+  p.parts = pieces(p.num_seqs, kThreads, 768);
 }
 int64_t verify_floats(const VerifyParams& p) {
-  return (int64_t)p.rows * p.pieces * (int64_t)(sizeof(Sum) / 4) + (int64_t)p.num_seqs * p.parts * 2 + p.num_seqs;
+  return (int64_t)p.rows * p.pieces * (int64_t)(sizeof(Sum) / 4) + (int64_t)p.num_seqs * 3;
 }
 int verify_sizes(const pkda_verify_args* a, VerifyParams& p) {
   PKDA_REQUIRE(a != nullptr, PKDA_EINVAL, "null args");
@@ -492,8 +549,8 @@ extern "C" int pkda_verify(const pkda_verify_args* a, void* stream) {
   p.cu = a->cu_seqlens; p.temperature = a->temperature; p.temperature_all = a->temperature_all;
   p.tokens = a->tokens; p.accepted = a->accepted;
   p.sums = reinterpret_cast<Sum*>(a->workspace);
-  p.best = reinterpret_cast<Best*>(p.sums + (int64_t)p.rows * p.pieces);
-  p.done = reinterpret_cast<int32_t*>(p.best + (int64_t)p.num_seqs * p.parts);
+  p.best = reinterpret_cast<uint64_t*>(p.sums + (int64_t)p.rows * p.pieces);
+  p.done = reinterpret_cast<int32_t*>(p.best + p.num_seqs);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 block(kThreads);
   if (p.rows > 0) {
