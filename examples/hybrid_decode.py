@@ -5,7 +5,9 @@ slot of every PKDA layer's pool and into pages of every attention layer's
 cache; then all live sequences decode together, one HIP graph replay a token,
 and the next token of each is drawn with its own settings.
 
-    python examples/hybrid_decode.py --seqs 64 --tokens 128
+    python examples/hybrid_decode.py --seqs 64 --tokens 128 [--fp8]
+
+With ``--fp8`` the attention layers norm their heads and keep 8-bit floats.
 
 The weights are random: the tokens mean nothing, the calls are the real ones.
 """
@@ -24,8 +26,9 @@ from torch.nn import functional as F
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
-from delta_feedback_experiment_amd import (DecodePool, PagedKV, paged_append_, paged_attention, pkda_decode_step_,
-                                           pkda_prefill_, pkda_qkv_conv_cached_, sample_tokens)
+from delta_feedback_experiment_amd import (DecodePool, PagedKV, PagedKVFP8, paged_append_, paged_append_fp8_,
+                                           paged_attention, paged_attention_fp8, pkda_decode_step_, pkda_prefill_,
+                                           pkda_qkv_conv_cached_, sample_tokens)
 
 
 @dataclass
@@ -40,6 +43,7 @@ class Sizes:
     pages: int = 1024        # of each attention layer's cache
     max_pages: int = 32      # of one sequence
     dtype: torch.dtype = torch.bfloat16
+    fp8: bool = False        # attention layers with head norms and a cache of 8-bit floats
 
 
 class Trunk:
@@ -63,9 +67,14 @@ class Trunk:
                     conv=torch.randn(3 * self.width, 4, generator=gen, device=device) * 0.5,
                     pool=DecodePool.zeros(s.slots, s.heads, s.head_dim, dtype=s.dtype, precond=False, device=device)))
             else:
+                size = (s.pages, s.page_size, s.kv_heads, s.head_dim)
                 self.layers.append(dict(
                     qkv=weight(self.width, (s.heads + 2 * s.kv_heads) * s.head_dim), out=out,
-                    cache=PagedKV.zeros(s.pages, s.page_size, s.kv_heads, s.head_dim, dtype=s.dtype, device=device)))
+                    cache=PagedKVFP8.zeros(*size, device=device) if s.fp8 else
+                    PagedKV.zeros(*size, dtype=s.dtype, device=device)))
+                if s.fp8:
+                    self.layers[-1]["norms"] = [1 + 0.1 * torch.randn(s.head_dim, generator=gen, device=device)
+                                                for _ in range(2)]
         angle = torch.outer(torch.arange(s.max_pages * s.page_size, device=device),
                             10000.0 ** (-torch.arange(0, s.head_dim, 2, device=device) / s.head_dim))
         self.cos, self.sin = angle.cos(), angle.sin()
@@ -86,8 +95,14 @@ class Trunk:
         s = self.s
         q, k, v = (h @ w["qkv"]).unflatten(-1, (-1, s.head_dim)).split((s.heads, s.kv_heads, s.kv_heads), 1)
         c = w["cache"]
-        q = paged_append_(k, v, c.k, c.v, table, lens, cu_seqlens=cu, q=q, cos=self.cos, sin=self.sin)
-        o, _ = paged_attention(q, c.k, c.v, table, lens, cu_seqlens=cu)
+        place = dict(cu_seqlens=cu, q=q, cos=self.cos, sin=self.sin)
+        if s.fp8:
+            q = paged_append_fp8_(k, v, c.k, c.v, c.k_scale, c.v_scale, table, lens, q_norm=w["norms"][0],
+                                  k_norm=w["norms"][1], **place)
+            o, _ = paged_attention_fp8(q, c.k, c.v, c.k_scale, c.v_scale, table, lens, cu_seqlens=cu)
+        else:
+            q = paged_append_(k, v, c.k, c.v, table, lens, **place)
+            o, _ = paged_attention(q, c.k, c.v, table, lens, cu_seqlens=cu)
         return o.flatten(1)
 
     def __call__(self, tokens: Tensor, slots: Tensor, table: Tensor, lens: Tensor, cu: Tensor | None = None) -> Tensor:
@@ -191,8 +206,9 @@ def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--seqs", type=int, default=64)
     ap.add_argument("--tokens", type=int, default=128)
+    ap.add_argument("--fp8", action="store_true")
     args = ap.parse_args()
-    s = Sizes(slots=args.seqs, pages=args.seqs * 32)
+    s = Sizes(slots=args.seqs, pages=args.seqs * 32, fp8=args.fp8)
     trunk = Trunk(s)
     dev = trunk.embed.device
     gen = torch.Generator().manual_seed(1)
