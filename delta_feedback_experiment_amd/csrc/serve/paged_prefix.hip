@@ -12,6 +12,9 @@
 // part takes whole tiles of keys; what is left of a prefix belongs to the
 // sequences' own part, so that no tile of keys lies on both sides.
 //
+// Which of a group's pages the shared positions are read from is this file's to
+// choose, since all of them hold the same there.
+//
 // A row whose position lies inside its group's prefix sees what is before it, as
 // it would without the group.
 #include "paged_attention.h"
@@ -57,9 +60,22 @@ inline PrefixPlan prefix_plan(AttnParams& shared, AttnParams& own) {
   return r;
 }
 
+// Sequences of more than 128 rows are tiles of their own, which read the shared
+// positions for as many rows as a group's tiles would; where those fill the card
+// nothing is left to gain by parts and their joining, and every sequence attends all
+// it holds.  16 sequences behind 4,096, 32/8 heads, 32 new tokens each: 94 us by parts
+// and 137 so, 48 tokens 156 and 139, 96 tokens 204 and 172; but 8 sequences of 48
+// behind 8,192 153 and 235, 4 of 96 behind 16,384 266 and 457.
+inline bool without_parts(const AttnParams& p) {
+  const int64_t S = p.s.num_seqs;
+  const int64_t per_seq = S > 0 ? ((int64_t)p.s.num_tokens * p.group.d + S - 1) / S : 0;
+  return per_seq > kRowTile && S * ((per_seq + kRowTile - 1) / kRowTile) * p.kv_heads >= kSlots / 2;
+}
+
 template <typename G>
 int launch_prefix(AttnParams shared, AttnParams own, hipStream_t s) {
   constexpr const char* what = "pkda_paged_prefix_attention";
+  if (without_parts(own)) return launch_attention<G>(own, s, what);
   const PrefixPlan r = prefix_plan(shared, own);
   const int64_t shared_tile = (int64_t)shared.kv_heads * shared.splits, own_tile = (int64_t)own.kv_heads * own.splits;
   const int64_t first = (r.shared.row_tiles + r.shared.key_tiles) * shared_tile;
@@ -108,6 +124,7 @@ extern "C" int64_t pkda_paged_prefix_workspace(const pkda_paged_prefix_args* a) 
   using namespace pkda;
   AttnParams shared;
   if (sizes_of(a, shared)) return -1;
+  if (without_parts(shared)) return attention_workspace(a, shared);
   // by the sizes alone: one token a sequence may come with cu_seqlens or without
   int splits = 0;
   for (const bool packed : {true, false}) {
@@ -134,9 +151,12 @@ extern "C" int pkda_paged_prefix_attention(const pkda_paged_prefix_args* a, void
   PKDA_REQUIRE(a->num_groups == 0 || (a->cu_groups && a->prefix_lens), PKDA_EINVAL, "null groups");
   if (a->num_tokens == 0) return 0;
   AttnParams own = shared;
-  prefix_plan(shared, own);
-  if (int st = attention_tensors(a, shared, vec, shared.splits + own.splits)) return st;
-  PKDA_REQUIRE(shared.part_o, PKDA_EINVAL, "workspace");
+  int parts = own.splits;
+  if (!without_parts(own)) {
+    prefix_plan(shared, own);
+    parts = shared.splits + own.splits;
+  }
+  if (int st = attention_tensors(a, shared, vec, parts)) return st;
   shared.k_scales = a->k_scales; shared.v_scales = a->v_scales;
   shared.k_scale_stride = a->k_scale_stride; shared.v_scale_stride = a->v_scale_stride;
   shared.groups = a->cu_groups; shared.prefix_lens = a->prefix_lens;

@@ -3,7 +3,7 @@ server holds twice the positions in, and a decode step reads in half the time.
 
 The pools are those of :mod:`.paged` with E4M3 codes (``float8_e4m3fn``) for
 numbers, and a scale for every 32 channels of a row (``float8_e8m0fnu``, a power
-of two): a key or value is ``code * scale``, which BF16 holds exactly.
+of two, 2^-117 .. 2^119): a key or value is ``code * scale``, which BF16 holds exactly.
 :func:`paged_append_fp8_` quantises the new tokens' keys and values as it stores
 them; :func:`paged_attention_fp8` is :func:`.paged.paged_attention` over the
 numbers that the cache stands for.  Tables, lengths and what they may say wrong

@@ -165,8 +165,9 @@ int pkda_sample(const pkda_sample_args* args, void* stream);
  * E4M3 codes (4 exponent bits, 3 mantissa bits, no infinity), and for each 32
  * channels of a row a scale 2^(e - 127) held as the byte e,
  * [num_pages, page_size, kv_heads, head_dim / 32], pages k_scale_stride /
- * v_scale_stride bytes apart.  A number is code * scale, exact in BF16 and FP32.
- * head_dim 64 or 128.
+ * v_scale_stride bytes apart.  A number is code * scale, exact in BF16 and FP32 for
+ * the scales that the store writes, bytes 10 .. 246; what others stand for where a
+ * sequence has a position is undefined.  head_dim 64 or 128.
  *
  * Store: pkda_paged_append with, on the way, the norms of query and key heads,
  * before the rotation (NULL: none):

@@ -255,6 +255,19 @@ def test_attention_of_long_and_many(dev, dtype, page):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S,Hkv", [(130, 4), (64, 8), (512, 1), (513, 1), (65, 8)])
+def test_single_tokens_of_many_sequences(dev, dtype, S, Hkv):
+    """As many as the card takes the longest first of, and more; equal lengths and none
+    among them."""
+    print(f"[gpu] fp8 decode, {S} sequences of {Hkv} heads {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(S)
+    lens = torch.randint(0, 90, (S,), generator=gen)
+    lens[::5], lens[3::7], lens[-1] = 40, 0, 300
+    Cache8(lens.tolist(), [1] * S, 2 * Hkv, Hkv, 64, 16, dtype, seed=S, cu=False).check(dev, long=True)
+    Cache8([33] * S, [1] * S, 2 * Hkv, Hkv, 64, 16, dtype, seed=S, cu=False).check(dev, long=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_attention_of_tokens_without_keys(dev, dtype):
     """Padding past cu_seqlens[-1], more new tokens than positions, missing pages."""
     print(f"[gpu] fp8 attention without keys {dtype}", flush=True)

@@ -164,9 +164,24 @@ def test_large_groups_of_many_rows(dev, dtype, eight, page):
     own = [n + (5 * i) % 40 for i, n in enumerate(new)]
     Batch([(333, 40), (700, 50)], own, new, 32, 8, 64, page, dtype, fp8_cache=eight, seed=5).check(dev)
     # rows enough that sequences' own part is tiles of 128 too
+    new = [8 + i for i in range(40)]
+    Batch([(450, 30), (77, 10)], [n + 3 * (i % 9) for i, n in enumerate(new)], new, 32, 8, 64, page, dtype,
+          fp8_cache=eight, seed=6).check(dev)
+    # and so many that every sequence is attended whole
     new = [64 + i for i in range(20)]
     Batch([(450, 20)], [n + 3 * i for i, n in enumerate(new)], new, 32, 8, 64, page, dtype, fp8_cache=eight,
           seed=6).check(dev)
+
+
+@pytest.mark.parametrize("groups", [62, 63, 64, 65, 130])
+def test_as_many_groups_as_lanes_and_more(dev, groups):
+    print(f"[gpu] prefix, {groups} groups", flush=True)
+    sizes = [(64 * (i % 4) + i % 7, 1 + i % 3) for i in range(groups)]
+    n = sum(c for _, c in sizes) + 3
+    own = [1 + i % 11 for i in range(n)]
+    for cu in (False, True):
+        new = [1 + i % 3 if cu else 1 for i in range(n)]
+        Batch(sizes, [o + x for o, x in zip(own, new)], new, 4, 2, 64, 16, torch.bfloat16, seed=groups, cu=cu, loose=3).check(dev)
 
 
 def test_heads_of_32_channels(dev):
