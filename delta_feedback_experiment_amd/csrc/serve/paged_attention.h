@@ -167,13 +167,6 @@ __device__ __forceinline__ int lds_chunk(int row, int chunk) {  // byte offset
 template <int RB>
 __device__ __forceinline__ int lds_row(int row) { return row * RB + (swizzle<RB>(row) << 4); }
 template <int RB> constexpr int kFlip8 = RB >= 256 ? 8 : 2;
-// A number the compiler cannot know, so that what follows from it is computed again
-// in every turn of a loop, by an operation each, and not kept in a register each.
-__device__ __forceinline__ int anew(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
 // acc += A B over one chunk pair; lane: row / column lane & 31, the half's chunk.
 template <typename T>
 __device__ __forceinline__ void mma_chunk(f32x16& acc, const u32x4& a, const u32x4& b) {
@@ -634,16 +627,10 @@ __device__ __forceinline__ Place place_of(unsigned block, unsigned blocks, int h
 // Up to 32 rows a tile: the keys over the waves.
 // ---------------------------------------------------------------------------
 template <typename G> struct KeysLds {
-  // the output is joined in JP pieces of its channels, which LDS holds one of
-  static constexpr int JP = G::FP8 ? 2 : 1, JD = G::D / JP;
-  static constexpr int OS = JD + 4;  // floats between the rows of a wave's piece
+  static constexpr int OS = G::D + 4;  // floats between the rows of a wave's output
   static constexpr int kStage = kWaves * 32 * G::RB, kJoin = kWaves * 32 * OS * 4;
   __align__(16) char buf[kStage > kJoin ? kStage : kJoin];
   float m[kWaves][32], l[kWaves][32];
-  // rows of 256 bytes and more of an 8-bit cache leave their queries here, where
-  // each product reads its operand: a third workgroup a compute unit for it
-  static constexpr bool kQueries = G::FP8 && G::RB >= 256;
-  __align__(16) char q[kQueries ? 32 * G::RB : 16];
 };
 
 template <typename G, Part PART>
@@ -709,18 +696,11 @@ __device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block,
     r = r1;
   }
   arrived(q);
-  constexpr bool kQueries = KeysLds<G>::kQueries;
   // this lane's row of operands in LDS: operand i is chunk(i, 0)'s bits away
   const int lrow = lds_row<G::RB>(col) ^ (G::chunk(0, half) << 4);
-  if constexpr (kQueries) {  // every wave the same numbers, so that none waits for another
-#pragma unroll
-    for (int i = 0; i < G::NP; ++i) *reinterpret_cast<u32x4*>(lds.q + (lrow ^ (G::chunk(i, 0) << 4))) = q[i];
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-  }
   for (int t = w; t < tiles; t += kWaves) {
     const int key0 = k0 + 32 * t;
     const uint32_t there = (uint32_t)__ballot(here);
-    const int at = kQueries ? anew(lrow) : lrow;
     f32x16 s[1];
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
@@ -729,13 +709,7 @@ __device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block,
       u32x4 x[G::M];
       expand<G>(k[i], (ks >> (8 * i)) & 0xff, x);
 #pragma unroll
-      for (int j = 0; j < G::M; ++j) {
-        const int o = G::M * i + j;
-        if constexpr (kQueries)
-          mma_chunk<T>(s[0], x[j], *reinterpret_cast<const u32x4*>(lds.q + (at ^ (G::chunk(o, 0) << 4))));
-        else
-          mma_chunk<T>(s[0], x[j], q[o]);
-      }
+      for (int j = 0; j < G::M; ++j) mma_chunk<T>(s[0], x[j], q[G::M * i + j]);
     }
     // values to LDS: rows that are not there as zeros, and in a tile that some
     // row sees only part of, whatever is not finite
@@ -758,7 +732,7 @@ __device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block,
 #pragma unroll
         for (int j = 0; j < G::M; ++j) {
           if (clear) any |= clear_nonfinite<T>(x[j]);
-          *reinterpret_cast<u32x4*>(sv + (at ^ (G::chunk(G::M * i + j, 0) << 4))) = x[j];
+          *reinterpret_cast<u32x4*>(sv + (lrow ^ (G::chunk(G::M * i + j, 0) << 4))) = x[j];
         }
       }
     } else {
@@ -767,7 +741,7 @@ __device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block,
         for (int i = 0; i < G::NP; ++i) any |= clear_nonfinite<T>(v[i]);
       }
 #pragma unroll
-      for (int i = 0; i < G::NP; ++i) *reinterpret_cast<u32x4*>(sv + (at ^ (G::chunk(i, 0) << 4))) = v[i];
+      for (int i = 0; i < G::NP; ++i) *reinterpret_cast<u32x4*>(sv + (lrow ^ (G::chunk(i, 0) << 4))) = v[i];
     }
     if (clear) {
       const uint64_t b = __ballot(any);
@@ -802,52 +776,45 @@ __device__ __forceinline__ void attend_keys(const AttnParams& p, unsigned block,
   }
   __syncthreads();
   const int live = min(32, tile.rows - tile.row0);
-  constexpr int JD = KeysLds<G>::JD;
+  {
+    float m = s_m[0][col];
 #pragma unroll
-  for (int part = 0; part < KeysLds<G>::JP; ++part) {
-    if (part) __syncthreads();
-    {
-      float m = s_m[0][col];
+    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, s_m[i][col]);
+    const float a = exp2_fast(run.m - (m == -INFINITY ? 0.f : m));
+    if (col < live) {
+      float* so = reinterpret_cast<float*>(s_buf) + (w * 32 + col) * OS;
 #pragma unroll
-      for (int i = 1; i < kWaves; ++i) m = fmaxf(m, s_m[i][col]);
-      const float a = exp2_fast(run.m - (m == -INFINITY ? 0.f : m));
-      if (col < live) {
-        float* so = reinterpret_cast<float*>(s_buf) + (w * 32 + col) * OS;
+      for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < JD / 32; ++dt) {
-          const f32x16& o = run.o[part * (JD / 32) + dt];
-#pragma unroll
-          for (int r = 0; r < 16; r += 4)
-            *reinterpret_cast<float4*>(so + 32 * dt + key_of(r, half)) =
-                make_float4(o[r] * a, o[r + 1] * a, o[r + 2] * a, o[r + 3] * a);
-        }
-      }
+        for (int r = 0; r < 16; r += 4)
+          *reinterpret_cast<float4*>(so + 32 * dt + key_of(r, half)) =
+              make_float4(run.o[dt][r] * a, run.o[dt][r + 1] * a, run.o[dt][r + 2] * a, run.o[dt][r + 3] * a);
     }
-    __syncthreads();
-    for (int x = threadIdx.x; x < live * (JD / 4); x += kThreads) {
-      const int i = x / (JD / 4), cp = 4 * (x % (JD / 4)), c = part * JD + cp;
-      float m = s_m[0][i];
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < live * (D / 4); x += kThreads) {
+    const int i = x / (D / 4), c = 4 * (x % (D / 4));
+    float m = s_m[0][i];
 #pragma unroll
-      for (int j = 1; j < kWaves; ++j) m = fmaxf(m, s_m[j][i]);
-      float sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 1; j < kWaves; ++j) m = fmaxf(m, s_m[j][i]);
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < kWaves; ++j) {
-        sum += s_l[j][i] * exp2_fast(s_m[j][i] - (m == -INFINITY ? 0.f : m));
-        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(s_buf) + (j * 32 + i) * OS + cp);
-        acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
-      }
-      const int r = tile.row0 + i, j = (int)p.group.div((uint32_t)r);
-      const int64_t out = (int64_t)(tile.span.first + j) * p.q_heads + kvh * (int)p.group.d + (r - j * (int)p.group.d);
-      if (tile.direct) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        store4(static_cast<T*>(p.o) + out * D + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-        if (c == 0) p.lse[out] = (m + __log2f(sum)) * 0.693147180559945309f;
-      } else {
-        const int64_t slot = (int64_t)split * p.s.num_tokens * p.q_heads + out;
-        *reinterpret_cast<float4*>(p.part_o + slot * D + c) = acc;
-        if (c == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m, sum);
-      }
+    for (int j = 0; j < kWaves; ++j) {
+      sum += s_l[j][i] * exp2_fast(s_m[j][i] - (m == -INFINITY ? 0.f : m));
+      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(s_buf) + (j * 32 + i) * OS + c);
+      acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
+    }
+    const int r = tile.row0 + i, j = (int)p.group.div((uint32_t)r);
+    const int64_t out = (int64_t)(tile.span.first + j) * p.q_heads + kvh * (int)p.group.d + (r - j * (int)p.group.d);
+    if (tile.direct) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      store4(static_cast<T*>(p.o) + out * D + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+      if (c == 0) p.lse[out] = (m + __log2f(sum)) * 0.693147180559945309f;
+    } else {
+      const int64_t part = (int64_t)split * p.s.num_tokens * p.q_heads + out;
+      *reinterpret_cast<float4*>(p.part_o + part * D + c) = acc;
+      if (c == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, sum);
     }
   }
 }

@@ -17,6 +17,8 @@
 //
 // A row whose position lies inside its group's prefix sees what is before it, as
 // it would without the group.
+#include <stddef.h>
+
 #include "paged_attention.h"
 
 namespace pkda {
@@ -72,10 +74,21 @@ inline bool without_parts(const AttnParams& p) {
   return per_seq > kRowTile && S * ((per_seq + kRowTile - 1) / kRowTile) * p.kv_heads >= kSlots / 2;
 }
 
+// The call without its groups: the plain attentions' arguments begin this one's.
+template <typename A>
+A whole_args(const pkda_paged_prefix_args* a) {
+  static_assert(offsetof(A, workspace) == offsetof(pkda_paged_prefix_args, workspace) &&
+                    sizeof(A) <= offsetof(pkda_paged_prefix_args, cu_groups),
+                "the same fields in the same places");
+  A b;
+  memcpy(&b, a, sizeof(b));
+  b.struct_size = (int32_t)sizeof(b);
+  return b;
+}
+
 template <typename G>
 int launch_prefix(AttnParams shared, AttnParams own, hipStream_t s) {
   constexpr const char* what = "pkda_paged_prefix_attention";
-  if (without_parts(own)) return launch_attention<G>(own, s, what);
   const PrefixPlan r = prefix_plan(shared, own);
   const int64_t shared_tile = (int64_t)shared.kv_heads * shared.splits, own_tile = (int64_t)own.kv_heads * own.splits;
   const int64_t first = (r.shared.row_tiles + r.shared.key_tiles) * shared_tile;
@@ -150,13 +163,17 @@ extern "C" int pkda_paged_prefix_attention(const pkda_paged_prefix_args* a, void
   }
   PKDA_REQUIRE(a->num_groups == 0 || (a->cu_groups && a->prefix_lens), PKDA_EINVAL, "null groups");
   if (a->num_tokens == 0) return 0;
-  AttnParams own = shared;
-  int parts = own.splits;
-  if (!without_parts(own)) {
-    prefix_plan(shared, own);
-    parts = shared.splits + own.splits;
+  if (without_parts(shared)) {
+    if (fp8) {
+      const auto b = whole_args<pkda_paged_attention_fp8_args>(a);
+      return pkda_paged_attention_fp8(&b, stream);
+    }
+    const auto b = whole_args<pkda_paged_attention_args>(a);
+    return pkda_paged_attention(&b, stream);
   }
-  if (int st = attention_tensors(a, shared, vec, parts)) return st;
+  AttnParams own = shared;
+  prefix_plan(shared, own);
+  if (int st = attention_tensors(a, shared, vec, shared.splits + own.splits)) return st;
   shared.k_scales = a->k_scales; shared.v_scales = a->v_scales;
   shared.k_scale_stride = a->k_scale_stride; shared.v_scale_stride = a->v_scale_stride;
   shared.groups = a->cu_groups; shared.prefix_lens = a->prefix_lens;
