@@ -90,8 +90,10 @@ def _check_cache(name: str, x: Tensor, k_pages: Tensor, v_pages: Tensor, page_ta
         if (stride[3] != 1 or (stride[2] != D and H > 1) or (stride[1] != H * D and R > 1)
                 or not _aligned(t, stride[0])) and t.numel():
             raise ValueError("every page must be dense, in whole 16 bytes")
-    for t in scales or ():
-        B = D // SCALE_BLOCK
+    if scales is None:
+        return
+    B = D // SCALE_BLOCK
+    for t in scales:
         if t.dtype != torch.float8_e8m0fnu or tuple(t.shape) != (P, R, H, B):
             raise ValueError(f"scales must be float8_e8m0fnu {(P, R, H, B)}, not {t.dtype} {tuple(t.shape)}")
         stride = t.stride()
@@ -220,6 +222,8 @@ def _check_append(k: Tensor, v: Tensor, k_pages: Tensor, page_table: Tensor, q: 
             raise ValueError(f"cos and sin hold {cos.shape[0]} positions, a row of page_table {capacity}")
     if q_norm is not None and q is None:
         raise ValueError("q_norm without q")
+    if q_norm is None and k_norm is None:
+        return
     for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
         if w is not None and (tuple(w.shape) != (k.shape[2],) or w.dtype not in (torch.float32, torch.bfloat16)):
             raise ValueError(f"{name} must be float32 or bfloat16 [{k.shape[2]}], not {w.dtype} {tuple(w.shape)}")
@@ -387,8 +391,10 @@ def _attend(struct, entry: str, sizes: str, device: torch.device, q: Tensor, k_p
         head_dim=D, page_size=k_pages.shape[1], max_pages=page_table.shape[1], num_pages=k_pages.shape[0],
         table_stride=page_table.stride(0), cu_seqlens=_ptr(cu_seqlens), seq_lens=_ptr(seq_lens),
         page_table=_ptr(page_table), q=_ptr(q), q_stride=q.stride(0), k_pages=_ptr(k_pages), v_pages=_ptr(v_pages),
-        k_page_stride=k_pages.stride(0), v_page_stride=v_pages.stride(0), scale=scale, o=_ptr(o), lse=_ptr(lse), **more,
+        k_page_stride=k_pages.stride(0), v_page_stride=v_pages.stride(0), scale=scale, o=_ptr(o), lse=_ptr(lse),
     )
+    for name, value in more.items():
+        setattr(args, name, value)
     if k_scales is not None:
         args.k_scales, args.v_scales = _ptr(k_scales), _ptr(v_scales)
         args.k_scale_stride, args.v_scale_stride = k_scales.stride(0), v_scales.stride(0)
