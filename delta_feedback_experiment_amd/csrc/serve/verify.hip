@@ -66,8 +66,11 @@ struct VerifyParams {
   int32_t* done;   // [num_seqs] how many those are
 };
 
+// One logit as the rows' vectors are taken: +inf is the largest number of its own type.
 template <typename T>
-__device__ __forceinline__ float one_logit(const T* l, int i) { return usable(io<T>::load(l + i)); }
+__device__ __forceinline__ float one_logit(const T* l, int i) {
+  return fminf(usable(io<T>::load(l + i)), __uint_as_float(sizeof(T) == 2 ? 0x7f7f0000u : 0x7f7fffffu));
+}
 
 __device__ __forceinline__ int row_bound(const VerifyParams& p, int n) {
   return n == 0 ? 0 : clamp_int(p.cu[n], 0, p.rows);

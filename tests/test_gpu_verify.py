@@ -132,6 +132,27 @@ def test_infinities_and_nan(dev):
             d.check(dev)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("draft", [True, False])
+def test_a_draft_at_an_infinite_logit(dev, dtype, draft):
+    """Several +inf share a row's probability evenly, the draft's among them."""
+    for temperature in (1.0, 0.3):
+        d = Drafts([2] * 40, 777, dtype, seed=31, draft=draft)
+        d.temperature = temperature
+        d.logits[:, 30] = d.logits[:, 60] = math.inf  # p = 1/2
+        d.drafts[:] = 30
+        d.uniform[::2] = torch.linspace(0.02, 0.98, 40)
+        if draft:
+            d.draft_logits[:, 30] = math.inf  # q = 1, or 1/4: accepted whatever the number
+            d.draft_logits[40:, [1, 2, 700]] = math.inf
+        print(f"[gpu] verify, drafts at +inf, T {temperature}", flush=True)
+        _, accepted = d.check(dev)
+        stands = (d.uniform[::2] < 0.5).int()
+        if draft:
+            stands[20:] = 1
+        assert torch.equal(accepted.cpu(), stands)
+
+
 @pytest.mark.parametrize("temperature", [math.inf, 1e-6, 1e-38, 1e-45, 30.0])
 def test_temperatures(dev, temperature):
     print(f"[gpu] verify, temperature {temperature}", flush=True)
