@@ -4,7 +4,8 @@
 // p = softmax(l / T) in the row after a draft's place, q the same of the draft's
 // own logits (or 1 at the draft).  Drafts are accepted in turn while u q(d) < p(d);
 // the next token maximises log max(p - q, 0) + noise in the first row whose draft
-// is not, log p + noise in the last row (the Gumbel numbers make that a draw).
+// is not, log p + noise in the last row and in one without a draft, where nothing was
+// drawn from q (the Gumbel numbers make that a draw).
 //
 // Bound by the logits' bytes.  Two launches.  The first reads every row of the
 // target and of the drafts once, a row over several workgroups, and leaves each
@@ -261,6 +262,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyParams p) {
 struct RowSum {
   float m, s, dm, ds;
   int first;
+  int drafted;  // lane 0's: the row's draft, -1 for none that can be taken
 };
 // f over the wave's x, every lane getting it.
 template <typename V, typename F>
@@ -305,6 +307,7 @@ __device__ __forceinline__ RowSum row_sum(const Sum& x, float c) {
   r.s = wave_total(x.s * carried(x.m, r.m, c));
   r.ds = wave_total(x.ds * carried(x.dm, r.dm, c));
   r.first = wave_min(x.m == r.m ? x.first : INT32_MAX);
+  r.drafted = x.drafted;
   return r;
 }
 __device__ __forceinline__ Best block_best(Best b, Best (&lds)[kWaves]) {
@@ -467,8 +470,8 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyParams p) {
     const T* q = draft ? draft + row * p.draft_stride : nullptr;
     const float* noise = p.noise + n * p.noise_stride;
     const bool rejected = stop + 1 < count;
-    const bool left = rejected && q;
-    const int without = rejected && !q ? p.drafts[row] : -1;
+    const bool left = rejected && q && r.drafted >= 0;  // (else nothing was drawn from q)
+    const int without = rejected && !q ? r.drafted : -1;
     Best b = block_best(scan_row<T>(p, l, q, noise, t, r, left, without, part, p.parts), s_best);
     if (p.parts > 1) {
       // The parts' best by one atomic maximum: nothing but atomics passes between

@@ -42,9 +42,9 @@ def verify_tokens(
     q[d] < p[d]``.  The next token is then the lowest index that maximises
     ``log(r) + noise`` over ``r > 0``: in the row of the first draft that is not
     accepted ``r = max(p - q, 0)`` (``p`` where that leaves nothing), in a
-    sequence's last row ``r = p``.  Drafts and next token together are draws from
-    the target alone.  ``temperature <= 0`` accepts a draft that is the (first)
-    largest logit's and takes that token next.
+    sequence's last row, and in one without a draft, ``r = p``.  Drafts and next
+    token together are draws from the target alone.  ``temperature <= 0`` accepts a
+    draft that is the (first) largest logit's and takes that token next.
 
     ``tokens [rows]`` int32: in a sequence's rows its accepted drafts, the next
     token, then -1; -1 in rows past ``cu_seqlens[-1]``.  ``accepted [S]`` int32
@@ -52,8 +52,8 @@ def verify_tokens(
 
     Logits of NaN or -inf have probability 0, +inf counts as the largest finite
     number: a top-k or top-p cut is made by -inf.  A draft outside the vocabulary
-    (-1: none) is not accepted.  A row that holds no logit accepts nothing and its
-    token is -1.
+    (-1: the row has none) is not accepted.  A row that holds no logit accepts nothing
+    and its token is -1.
     """
     given = [t for t in (temperature,) if isinstance(t, Tensor)]
     _require_device(logits, drafts, uniform, noise, cu_seqlens, draft_logits, *given)

@@ -295,13 +295,14 @@ int pkda_paged_prefix_attention(const pkda_paged_prefix_args* args, void* stream
  * drafts are accepted in turn while  uniform q(d) < p(d).  The token after the
  * accepted ones is the lowest index that maximises log r + noise over r > 0, r =
  * max(p - q, 0) in the row of the first draft that is not accepted (p where that
- * is nowhere positive), p in the last row.  temperature <= 0 accepts a draft that
- * is the lowest index of the largest logit, and takes that as the next token.
+ * is nowhere positive), p in the last row and in one whose draft is outside the
+ * vocabulary, where nothing was drawn from q.  temperature <= 0 accepts a draft
+ * that is the lowest index of the largest logit, and takes that as the next token.
  * An infinite temperature makes p and q even over what has a logit.
  *
  * NaN and -inf logits have p = 0 (q = 0); +inf counts as the largest finite
- * number.  A draft outside the vocabulary is not accepted.  A row without any
- * other logit accepts nothing and its token is -1.
+ * number.  A draft outside the vocabulary (none) is not accepted.  A row without
+ * any other logit accepts nothing and its token is -1.
  * tokens[row] is the row's draft where that was accepted, the next token in the
  * row after those, and -1 in the others (and in rows of no sequence).
  * ------------------------------------------------------------------------- */

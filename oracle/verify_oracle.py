@@ -68,14 +68,15 @@ def check(tokens: Tensor, accepted: Tensor, logits, drafts, uniform, noise, cu, 
                 seen[row] = d
                 continue
             token = int(tokens[row])
-            rest = p if last else (p - q).clamp(min=0)
+            # (without a draft nothing was drawn from q)
+            rest = p if last or not inside else (p - q).clamp(min=0)
             if not (rest > 0).any():
                 rest = p
             if not (rest > 0).any():
                 assert token == -1, (n, j, token)
                 continue
             score = rest.log() + noise[n].double()
-            off = slack * (1 + (p + (0 if last else q)) / rest.clamp(min=1e-300))
+            off = slack * (1 + (p + (0 if last or not inside else q)) / rest.clamp(min=1e-300))
             off = torch.where(rest > 0, off, 0.0)
             assert 0 <= token < p.numel() and rest[token] > 0, (n, j, token)
             assert score[token] + off[token] >= (score - off)[rest > 0].max(), (n, j, token, int(score.argmax()))
