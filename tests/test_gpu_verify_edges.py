@@ -1,4 +1,5 @@
-"""Verification where a row has no draft though draft logits are given, on the GPU.
+"""Verification where a row has no draft though draft logits are given, and at
+temperatures whose reciprocal is past FP32, on the GPU.
 
 The oracle's bars are those of ``test_gpu_verify.py``; the rest is exact.
 """
@@ -85,3 +86,28 @@ def test_draws_of_sequences_with_and_without_drafts(dev):
         chi = float(((torch.bincount(part.long(), minlength=V) - want) ** 2 / want).sum())
         print(f"[gpu] verify draws with and without drafts: chi-square {chi:.1f}", flush=True)
         assert chi < 40
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1e-6, 1e-38, 1e-45])
+def test_cold_drafts_stand_where_they_are_the_largest(dev, dtype, temperature):
+    """At the smallest temperatures p is 1 at the largest logit: a draft there stands
+    whatever the number (q <= 1), any other falls."""
+    for draft in (True, False):
+        print(f"[gpu] verify, cold {temperature} {dtype} draft logits {draft}", flush=True)
+        d = Drafts([3] * 9, 700, dtype, seed=40, draft=draft)
+        d.temperature = temperature
+        top = d.logits.float().sort(-1)
+        d.logits[torch.arange(27), top.indices[:, -1]] += 1  # (BF16 rows may tie at the top)
+        best = top.indices[:, -1].int()
+        d.drafts = best.clone()
+        d.uniform[:] = 1 - 2.0 ** -24
+        tokens, accepted = d.check(dev)
+        assert (accepted == 2).all() and torch.equal(tokens.cpu(), best)
+        wrong = torch.tensor([3 * n + n % 3 for n in range(9)])
+        d.drafts[wrong] = (best[wrong] + 1) % 700
+        if draft:  # the draft's own largest
+            d.draft_logits[wrong, d.drafts[wrong].long()] = 50.0
+        tokens, accepted = d.check(dev)
+        assert accepted.tolist() == [n % 3 for n in range(9)]
+        assert torch.equal(tokens.cpu()[wrong], best[wrong])
