@@ -258,7 +258,7 @@ __device__ __forceinline__ bool clear_nonfinite(u32x4& x) {
 struct Tile {
   SeqSpan span;
   int n, row0, rows;  // rows: of the sequence, from its first new token; n: whose pages
-  int seq_end;        // kShared: the group's sequences are n .. seq_end - 1
+  int seq0, seq_end;  // kShared: the group's sequences are seq0 .. seq_end - 1
   int first, last;    // positions of the tile's first and last row (negative: none)
   int begin, keys;    // what the tile sees: positions begin .. keys - 1
   int chunk;          // keys of a split
@@ -288,6 +288,41 @@ __device__ __forceinline__ int group_bound(const AttnParams& p, int g) {
 __device__ __forceinline__ int token_bound(const PagedSeqs& s, int n) {
   return n == 0 ? 0 : s.cu ? clamp_int(s.cu[n], 0, s.num_tokens) : n;
 }
+// f over the wave's x.
+template <typename F>
+__device__ __forceinline__ int wave_join(int x, F f) {
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false));   // quad [1,0,3,2]
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false));   // quad [2,3,0,1]
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false));  // half-row mirror
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false));  // row mirror
+  auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = f((int)r[0], (int)r[1]);
+  r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __builtin_amdgcn_readfirstlane(f((int)r[0], (int)r[1]));
+}
+__device__ __forceinline__ int wave_sum(int x) {
+  return wave_join(x, [](int a, int b) { return a + b; });
+}
+
+// A sequence of seq0 .. end - 1 that holds `want` positions, or where none does the
+// longest: past its length a sequence's row of the table names nothing of its own (a
+// slot that is finished is one of length 0), and none of the group's rows sees past
+// the longest's.  By the whole wave.
+__device__ __forceinline__ int holder_of(const PagedSeqs& s, int seq0, int end, int want) {
+  const int lane = threadIdx.x & 63;
+  int at = seq0, most = 0;
+  for (int n = seq0; n < end; n += 64) {
+    const int len = n + lane < end ? s.lens[n + lane] : -1;
+    const uint64_t whole = __ballot(len >= want);
+    if (whole) return n + __builtin_ctzll(whole);
+    const int longest = wave_join(len, [](int a, int b) { return max(a, b); });
+    if (longest > most) {
+      most = longest;
+      at = n + __builtin_ctzll(__ballot(len == longest));
+    }
+  }
+  return at;
+}
 // The positions that sequence n shares with its group (none without one).
 __device__ __forceinline__ int shared_of_seq(const AttnParams& p, int n) {
   const int g = wave_upper(p.num_groups, n, [&](int i) -> int64_t { return group_bound(p, i); });
@@ -306,8 +341,8 @@ __device__ __forceinline__ int token_position(const PagedSeqs& s, int t, int n, 
   return t - span.first < span.count ? max(-1, span.len - span.count + (t - span.first)) : -1;
 }
 
-// Tile `local` of M rows of sequence tile.n, whose span is given (kShared: of the
-// group whose first sequence it is; len is what the group shares).
+// Tile `local` of M rows of sequence tile.n, whose span is given (kShared: of a group
+// of whose sequences it is one; len is what the group shares).
 template <int M, Part PART = kAll>
 __device__ __forceinline__ bool fill_tile(const AttnParams& p, int local, const SeqSpan& span, Tile& tile) {
   const int group = (int)p.group.d;
@@ -353,13 +388,14 @@ __device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& 
       local = (int)(t - begin(g));
     }
     if (g >= p.num_groups) return false;
-    tile.n = __builtin_amdgcn_readfirstlane(group_bound(p, g));
+    tile.seq0 = __builtin_amdgcn_readfirstlane(group_bound(p, g));
     tile.seq_end = __builtin_amdgcn_readfirstlane(group_bound(p, g + 1));
-    if (tile.seq_end <= tile.n) return false;
+    if (tile.seq_end <= tile.seq0) return false;
     SeqSpan span;
-    span.first = token_bound(p.s, tile.n);
+    span.first = token_bound(p.s, tile.seq0);
     span.count = max(0, token_bound(p.s, tile.seq_end) - span.first);
-    span.len = shared_len(p, g);
+    span.len = __builtin_amdgcn_readfirstlane(shared_len(p, g));
+    tile.n = __builtin_amdgcn_readfirstlane(holder_of(p.s, tile.seq0, tile.seq_end, span.len));
     return fill_tile<M, kShared>(p, local, span, tile);
   }
   if (M == 32 && p.s.cu && p.key_rows == 32) {  // one tile a sequence
@@ -377,22 +413,6 @@ __device__ __forceinline__ bool find_tile(const AttnParams& p, int64_t t, Tile& 
     local = (int)(t - (int64_t)tile.n * per);
   }
   return fill_tile<M, PART>(p, local, seq_span(p.s, tile.n), tile);
-}
-
-// f over the wave's x.
-template <typename F>
-__device__ __forceinline__ int wave_join(int x, F f) {
-  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false));   // quad [1,0,3,2]
-  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false));   // quad [2,3,0,1]
-  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false));  // half-row mirror
-  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false));  // row mirror
-  auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  x = f((int)r[0], (int)r[1]);
-  r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  return __builtin_amdgcn_readfirstlane(f((int)r[0], (int)r[1]));
-}
-__device__ __forceinline__ int wave_sum(int x) {
-  return wave_join(x, [](int a, int b) { return a + b; });
 }
 
 // The t-th of the M-row tiles of sequences of more than key_rows rows, those
@@ -450,7 +470,7 @@ __device__ __forceinline__ Row load_row(const AttnParams& p, const Tile& tile, i
     const int j = (int)p.group.div((uint32_t)r), g = r - j * (int)p.group.d;
     const int h = kvh * (int)p.group.d + g, t = tile.span.first + j;
     row.index = (int64_t)t * p.q_heads + h;
-    if constexpr (PART == kShared) row.pos = min(tile.last, token_position(p.s, t, tile.n, tile.seq_end));
+    if constexpr (PART == kShared) row.pos = min(tile.last, token_position(p.s, t, tile.seq0, tile.seq_end));
     else row.pos = max(-1, tile.span.len - tile.span.count + j);
     const T* src = static_cast<const T*>(p.q) + t * p.q_stride + (int64_t)h * G::D;
 #pragma unroll

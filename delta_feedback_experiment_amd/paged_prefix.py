@@ -47,7 +47,9 @@ def paged_prefix_attention(
     of them, zero too): the same keys and values, in the same pages or in copies.
     Every sequence's row of ``page_table`` names the pages of all its positions,
     the shared ones too; from which of a group's rows those are read is not said.
-    Sequences past ``cu_groups[-1]`` share nothing.  Otherwise arguments and result
+    One that holds fewer positions than the prefix (a finished slot, of length 0) sees
+    what it holds of it and takes nothing from the others, whatever its row says past
+    its length; ``check_pages`` refuses it.  Sequences past ``cu_groups[-1]`` share nothing.  Otherwise arguments and result
     are those of :func:`.paged.paged_attention`, or with ``k_scales, v_scales`` of
     :func:`.paged_fp8.paged_attention_fp8`; both read the groups on the device, so
     that a captured step follows them.

@@ -249,8 +249,11 @@ int pkda_paged_attention_fp8(const pkda_paged_attention_fp8_args* args, void* st
  * cu_groups[g] .. cu_groups[g+1] - 1 (int32 [num_groups + 1], device; cu_groups[0]
  * counts as 0, bounds are clamped to num_seqs, sequences past the last share
  * nothing) hold the same keys and values at positions 0 .. prefix_lens[g] - 1,
- * in the same pages or in copies: which of the sequences' pages those are read
- * from is not said.  The result is that of pkda_paged_attention.
+ * in the same pages or in copies: from the pages of which of the sequences that
+ * hold a position it is read is not said.  A sequence of fewer positions than the
+ * prefix (a slot that is finished, of none) sees what it holds of it; the others see
+ * all of it, wherever that one stands in the group and whatever its row of the table
+ * says past its length.  The result is that of pkda_paged_attention.
  * ------------------------------------------------------------------------- */
 typedef struct pkda_paged_prefix_args {
   int32_t struct_size;
