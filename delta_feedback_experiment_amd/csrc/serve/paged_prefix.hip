@@ -17,8 +17,15 @@
 //
 // A row whose position lies inside its group's prefix sees what is before it, as
 // it would without the group.
-#include <stddef.h>
-
+//
+// Parts are taken whatever the numbers of new tokens, which the host does not know a
+// sequence at a time: by their mean one long chunk would decide for the sequences that
+// decode beside it.  Those are what parts are for (32/8 heads, us by parts and each
+// sequence whole: 60 of one token and one of 1,920 behind 16,384 682 and 1,037, one of
+// 3,900 1,398 and 1,742; 250 and one of 8,192 behind 8,192 2,118 and 2,750).  Long
+// chunks alone are better off whole, which their caller can have from the plain
+// attention (16 sequences behind 4,096, 33 tokens each 146 and 131, 96 tokens 198 and
+// 168, 512 tokens 874 and 689: two parts of a row are 2 x 1 KB of FP32 a head).
 #include "paged_attention.h"
 
 namespace pkda {
@@ -60,30 +67,6 @@ inline PrefixPlan prefix_plan(AttnParams& shared, AttnParams& own) {
   most = most < 1 ? 1 : most < kMaxSplits / 2 ? most : kMaxSplits / 2;
   if (own.splits > most) own.splits = (int)most;
   return r;
-}
-
-// Sequences of more than 128 rows are tiles of their own, which read the shared
-// positions for as many rows as a group's tiles would; where those fill the card
-// nothing is left to gain by parts and their joining, and every sequence attends all
-// it holds.  16 sequences behind 4,096, 32/8 heads, 32 new tokens each: 94 us by parts
-// and 137 so, 48 tokens 156 and 139, 96 tokens 204 and 172; but 8 sequences of 48
-// behind 8,192 153 and 235, 4 of 96 behind 16,384 266 and 457.
-inline bool without_parts(const AttnParams& p) {
-  const int64_t S = p.s.num_seqs;
-  const int64_t per_seq = S > 0 ? ((int64_t)p.s.num_tokens * p.group.d + S - 1) / S : 0;
-  return per_seq > kRowTile && S * ((per_seq + kRowTile - 1) / kRowTile) * p.kv_heads >= kSlots / 2;
-}
-
-// The call without its groups: the plain attentions' arguments begin this one's.
-template <typename A>
-A whole_args(const pkda_paged_prefix_args* a) {
-  static_assert(offsetof(A, workspace) == offsetof(pkda_paged_prefix_args, workspace) &&
-                    sizeof(A) <= offsetof(pkda_paged_prefix_args, cu_groups),
-                "the same fields in the same places");
-  A b;
-  memcpy(&b, a, sizeof(b));
-  b.struct_size = (int32_t)sizeof(b);
-  return b;
 }
 
 template <typename G>
@@ -137,7 +120,6 @@ extern "C" int64_t pkda_paged_prefix_workspace(const pkda_paged_prefix_args* a) 
   using namespace pkda;
   AttnParams shared;
   if (sizes_of(a, shared)) return -1;
-  if (without_parts(shared)) return attention_workspace(a, shared);
   // by the sizes alone: one token a sequence may come with cu_seqlens or without
   int splits = 0;
   for (const bool packed : {true, false}) {
@@ -163,14 +145,6 @@ extern "C" int pkda_paged_prefix_attention(const pkda_paged_prefix_args* a, void
   }
   PKDA_REQUIRE(a->num_groups == 0 || (a->cu_groups && a->prefix_lens), PKDA_EINVAL, "null groups");
   if (a->num_tokens == 0) return 0;
-  if (without_parts(shared)) {
-    if (fp8) {
-      const auto b = whole_args<pkda_paged_attention_fp8_args>(a);
-      return pkda_paged_attention_fp8(&b, stream);
-    }
-    const auto b = whole_args<pkda_paged_attention_args>(a);
-    return pkda_paged_attention(&b, stream);
-  }
   AttnParams own = shared;
   prefix_plan(shared, own);
   if (int st = attention_tensors(a, shared, vec, shared.splits + own.splits)) return st;

