@@ -23,7 +23,9 @@
 // and join at the end; keys go straight from memory to operand registers, values
 // through a wave's own piece of LDS (the transposing reads), the next tile's
 // loads in flight during a tile's arithmetic.  More rows (a chunk): four waves of
-// 32 rows share tiles of 64 keys staged in LDS, double-buffered.  Where rows are
+// 32 rows share tiles of 64 keys staged in LDS, double-buffered.  A third, the first
+// in 16x16 tiles, takes one token a sequence of up to 16 rows, given without
+// cu_seqlens, over an 8-bit cache and beside shared prefixes.  Where rows are
 // few, a sequence's keys are split over workgroups and a second kernel joins the
 // parts.
 //
@@ -33,13 +35,18 @@
 // What bounds it, measured in BF16 with heads of 128 (a large read runs at 4.0 to
 // 5.0 TB/s, a large matrix product at 1188 TFLOP/s).  Decode, 256 sequences of
 // 2,600 keys, 32/8 heads: 546 us, 4.98 TB/s of keys and values.  One sequence of
-// 131,072 keys: 114 us, 4.7 TB/s.  2,048 tokens after 14,336, 32/8 heads: 603 us,
-// 855 TFLOP/s: a wave's 32 products a tile are 1,024 cycles, its 246 vector
+// 131,072 keys: 114 us, 4.7 TB/s.  2,048 tokens after 14,336, 32/8 heads: 595 to 624
+// us by box, 825 to 865 TFLOP/s: a wave's 32 products a tile are 1,024 cycles, its 246 vector
 // instructions, 32 exponentials among them, about 1,370, and its reads of LDS
 // about 800; the other workgroup's wave on the SIMD overlaps them only in part
 // (2,500 cycles a tile and wave).  13 prompts of 250 to 1,659 tokens, 16/4 heads:
-// 87 us, 588 TFLOP/s: 6 us of a row tile's 33 are its way to its first keys and
-// its output.
+// 86 to 92 us by box, 560 to 591 TFLOP/s: 6 us of a row tile's 33 are its way to its
+// first keys and its output.
+//
+// Registers.  Of 256 a lane the 128-row form over an 8-bit cache, heads of 128, spills 7
+// and reloads three of them in every tile of keys (4 and none where a wave's staged rows
+// may lie in several pages; with shared prefixes it spills 6 and 3), and FP32 heads of 64
+// spill up to 4.
 #pragma once
 
 #include <math.h>
@@ -484,7 +491,9 @@ __device__ __forceinline__ Row load_row(const AttnParams& p, const Tile& tile, i
   return row;
 }
 // The queries arrive before the loop over the keys, and after the first keys are
-// asked for: waits inside the loop would hold the keys that are on their way.
+// asked for: waits inside the loop would hold the keys that are on their way.  (A
+// group's shared part asks for its keys after its rows' positions, whose lowest and
+// highest it needs.)
 template <int N>
 __device__ __forceinline__ void arrived(u32x4 (&q)[N]) {
 #pragma unroll

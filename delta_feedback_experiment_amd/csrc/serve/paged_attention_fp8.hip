@@ -12,8 +12,12 @@
 // What bounds it, in BF16 with heads of 128 (a 4 GiB copy runs at 4.55 TB/s).
 // Decode, 256 sequences of 325 to 4,875 keys, 32/8 heads: 288 us, 4.95 TB/s of codes
 // and scales (547 us over a BF16 cache).  4 sequences of 700 keys: 5.9 us and 3.6 for
-// the join, a trip to memory after the other.  2,048 tokens after 14,336: 600 us, 857
-// TFLOP/s, what the same takes over a BF16 cache: softmax beside products.
+// the join, a trip to memory after the other.  2,048 tokens after 14,336: 598 to 626 us
+// by box, 823 to 861 TFLOP/s, what the same takes over a BF16 cache: softmax beside
+// products.  Several new tokens, or one with cu_seqlens, run in the 32-row form in the
+// caller's order: those 256 sequences with one token so 349 us (4.2 TB/s), with five
+// 370 (3.9; 630 over a BF16 cache); 64 of them with five 124 (3.0; 192).  FP32 queries:
+// 465 us with one token, 1,228 where that comes with cu_seqlens, 1,266 with five.
 #include "paged_attention.h"
 
 namespace pkda {

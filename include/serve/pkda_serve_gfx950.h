@@ -292,7 +292,7 @@ int pkda_paged_prefix_attention(const pkda_paged_prefix_args* args, void* stream
  * clamped and cu_seqlens[0] 0 as above): row j of them holds the target's logits
  * after the sequence's first j drafts, and drafts[row], its uniform number and
  * its draft_logits (those the draft was drawn from) are of the draft after that
- * place; the last row has none, and what its entries hold is not read.  With
+ * place; the last row has none, whatever its entries hold.  With
  *   p = softmax(l / temperature),  q = softmax(draft l / temperature), or 1 at the
  *   draft and 0 elsewhere where draft_logits is NULL,
  * drafts are accepted in turn while  uniform q(d) < p(d).  The token after the
