@@ -83,6 +83,9 @@ def paged_append_fp8_(
     if check_pages:
         validate_pages(page_table, seq_lens, cu_seqlens, k.shape[0], k_pages.shape[0], k_pages.shape[1],
                        appended=True)
+    if torch.compiler.is_compiling():
+        # as the bytes they are: the compiler's default backend cannot have float8_e8m0fnu written in place
+        k_scales, v_scales = k_scales.view(torch.uint8), v_scales.view(torch.uint8)
     out = _registry.launch(store_op, k, v, k_pages, v_pages, k_scales, v_scales, page_table, seq_lens, cu_seqlens, q,
                            cos, sin, bool(interleaved), q_norm, k_norm, float(eps))
     return None if q is None else out
