@@ -13,7 +13,9 @@
 // sequences' own part, so that no tile of keys lies on both sides.
 //
 // Which of a group's pages the shared positions are read from is this file's to
-// choose, since all of them hold the same there.
+// choose, since all of the sequences that hold them hold the same there: the first
+// such sequence's, which a wave finds by 64 lengths at a time (under 1 us of a
+// tile's way to its keys).
 //
 // A row whose position lies inside its group's prefix sees what is before it, as
 // it would without the group.
